@@ -181,6 +181,40 @@ int rn_matrix_padded_columns(const rn_matrix* m, int* padded);
  * (walsh.rs:41-80). Codebook matrices only. Device pointers. */
 int rn_matrix_prepare(const rn_matrix* m, const float* x, int count, float* rotated, void* stream);
 
+/* ---- caches in device memory ------------------------------------------------------ */
+enum { RN_F32 = 0, RN_F16 = 1 };
+enum { RN_CACHE_F16 = 0, RN_CACHE_I8 = 1 };
+
+/* Keys and values of `sequences` x `kv_heads` x `capacity` positions, rows of 64.
+ * Row number r = sequence * sequence_rows + head * head_rows + position:
+ *   RN_CACHE_F16: keys and values hold fp16 bits, row r at element 64 r;
+ *   RN_CACHE_I8:  int8 codes, row r at element 64 r, and one f32 scale a row at
+ *                 element r of key_scales / value_scales.
+ * Contiguous caches have head_rows = capacity, sequence_rows = kv_heads * capacity;
+ * other orders and gaps are strides, as long as no two rows coincide. keys and values
+ * aligned to 16 bytes. At most 65535 sequences, 1024 heads, 2^24 positions. The
+ * caches of the sessions have these layouts (rn_session_layer_cache and the like). */
+typedef struct {
+    int format, sequences, kv_heads, capacity;
+    int64_t sequence_rows, head_rows;
+    void* keys;
+    void* values;
+    float* key_scales; /* null for RN_CACHE_F16 */
+    float* value_scales;
+} rn_cache;
+
+/* Rows outside a cache: row (sequence, token, head) of keys and of values starts at
+ * element sequence * sequence_stride + token * token_stride + head * head_stride and
+ * holds 64 values. So the k and v columns of a fused product's output are read in
+ * place (token_stride its row length), or another cache's rows (token_stride 64).
+ * Rows are aligned to 16 bytes: strides are multiples of 4 (f32) or 8 (f16). */
+typedef struct {
+    int type; /* RN_F32 or RN_F16 */
+    void* keys;
+    void* values;
+    int64_t sequence_stride, token_stride, head_stride;
+} rn_cache_rows;
+
 /* ---- the .cact archive (crates/cact; docs/format.md) ---------------------------
  * A memory-mapped, little-endian archive: 196-byte header, codebook levels, a
  * directory of 44-byte tensor records, 64-byte aligned blobs. Host-side; the
@@ -312,6 +346,8 @@ int rn_n3_session_pooled_readout(rn_n3_session* session, int code, float* out, i
  * ladder selection (whose cache the reference never fills). */
 int rn_n3_session_cache(rn_n3_session* session, int layer, int8_t* keys, float* key_scales, int8_t* values,
                         float* value_scales);
+/* rn_session_layer_cache of an active layer (RN_CACHE_I8). */
+int rn_n3_session_layer_cache(const rn_n3_session* session, int layer, rn_cache* out);
 int rn_n3_session_stream(const rn_n3_session* session, void** stream);
 
 /* ---- the depth ladder (crates/model/src/ladder.rs) -------------------------------
@@ -365,6 +401,97 @@ int rn_zero_centred_norm(const float* x, const float* gain, int count, int n, fl
  * stride), out [count][head_dim]. head_dim must be 64. Device pointers. */
 int rn_attend_heads(const float* q, const uint16_t* K, const uint16_t* V, const int32_t* lengths,
                     int count, int stride, int head_dim, float* out, void* stream);
+
+/* ---- serving over caller-held caches ---------------------------------------------
+ * What a server of these models runs besides the sessions: rows of a batch written
+ * into 8-bit or fp16 caches it holds itself, attention of a batch over one shared
+ * prefix (the reference clones a base session per turn, generator.rs:41-46, and reads
+ * the system prompt's cache again for every one of them), and the verification of
+ * drafted tokens. No counterpart in the reference beyond the arithmetic cited below.
+ *
+ * Every pointer is device memory of the stream's device (of the current device for
+ * the default stream); host arrays, other devices' memory and misaligned pointers are
+ * RN_ERR_ARGUMENT. The calls only enqueue kernels on `stream`: they allocate nothing,
+ * do not wait and may be captured into a graph. Numbers in device memory (starts,
+ * counts, lengths, ...) are read when the kernels run; a sequence whose numbers are
+ * out of range is left out, as each call says, and *error (nullable int32, which the
+ * calls never clear) becomes RN_ERR_ARGUMENT. */
+
+/* Writes `tokens` rows of every sequence and head into the cache, token t at position
+ * starts[sequence] + t. starts (nullable: 0) and counts (nullable: `tokens`) are
+ * device arrays [sequences]; of sequence b only the first counts[b] tokens are
+ * written, everything else stays as it is. 8-bit rows are ops::quantise_int8
+ * (ops.rs:103-118): scale = peak / 127 (1 where the peak is not positive; NaN does
+ * not count towards it), code = round(x / scale) half to even, NaN as 0 - bit for bit
+ * what rn_quantise_int8 and the int8 sessions compute. fp16 rows are rounded to
+ * nearest even. A sequence with counts[b] outside 0..tokens or rows outside the cache
+ * is not written. Source rows may repeat (strides of 0). */
+int rn_cache_write(const rn_cache* cache, const rn_cache_rows* rows, int tokens, const int32_t* starts,
+                   const int32_t* counts, int32_t* error, void* stream);
+/* The reverse: rows[.., t, ..] = the cache's rows at starts[b] + t, code * scale in
+ * f32 (rounded once more to fp16 for RN_F16). Tokens past counts[b] stay as they are. */
+int rn_cache_read(const rn_cache* cache, const rn_cache_rows* rows, int tokens, const int32_t* starts,
+                  const int32_t* counts, int32_t* error, void* stream);
+
+/* Attention of a batch: `sequences` sequences whose first prefix_length positions are
+ * one shared cache (sequence 0 of `prefix`; null with prefix_length 0) and whose
+ * further lengths[b] positions are sequence b of `own` (null: none, lengths null too;
+ * lengths null: the full capacity). The prefix is read once for all of them.
+ *   q   [sequences * queries] rows of [heads][64] f32, q_stride floats apart, rotated;
+ *   out [sequences * queries] rows of [heads][64] f32, out_stride floats apart.
+ * heads is a multiple (1..64) of the caches' kv_heads: query head h reads key head
+ * h * kv_heads / heads. Sequence b has counts[b] (nullable: `queries`) queries, which
+ * are the last counts[b] of its prefix_length + lengths[b] positions (tokens just
+ * written, such as drafted ones). The query at position p sees positions
+ * max(0, p + 1 - window)..p (window 0: from 0; attention.rs:171-177). With `score` the
+ * scale times q . k, out = sum softmax(score) v; a query that sees nothing gives
+ * zeros. Rows past counts[b] stay as they are. Positions a query does not see never
+ * reach it, whatever they hold; a NaN or infinity that it sees makes its output so.
+ * scale must be positive and finite.
+ * Products and sums are f32 (queries and weights enter the matrix instructions as
+ * pairs of fp16 numbers, 22 bits; relative error about 1e-6); the result depends on
+ * the shapes and lengths only and repeats bit for bit.
+ * A sequence with lengths[b] outside 0..capacity or counts[b] outside 0..queries gets
+ * NaN in all its rows. workspace: workspace_bytes of device memory aligned to 256
+ * bytes, at least what rn_attend_shared_workspace says for the same arguments; its
+ * contents need not be kept, and calls that may run at the same time (two streams, two
+ * graphs) need one each. At most 2^20 rows sequences * queries * heads. */
+int rn_attend_shared_workspace(int sequences, int queries, int heads, const rn_cache* prefix, int prefix_length,
+                               const rn_cache* own, size_t* bytes);
+int rn_attend_shared(const float* q, int64_t q_stride, float* out, int64_t out_stride, int sequences, int queries,
+                     int heads, const rn_cache* prefix, int prefix_length, const rn_cache* own,
+                     const int32_t* lengths, const int32_t* counts, float scale, int window, void* workspace,
+                     size_t workspace_bytes, int32_t* error, void* stream);
+
+/* Verification of drafted tokens (speculative decoding), from given random numbers.
+ *   target [sequences][drafts + 1] rows of `vocab` f32 logits, target_stride floats
+ *          apart: row i is what the target says after i of the drafted tokens;
+ *   draft  [sequences][drafts] rows of the model that drafted (draft_stride), or null:
+ *          the drafted tokens are taken as certain (a greedy or looked-up draft);
+ *   tokens [sequences][drafts] drafted; counts [sequences] (nullable: `drafts`) of them
+ *          are there; temperatures [sequences] (nullable: 1);
+ *   uniforms [sequences][drafts + 1] in [0, 1): of each drafted token, then of the draw.
+ * With p_i, q_i = softmax(logits / temperature) (-infinity masks a token), token i is
+ * accepted while u_i q_i(x_i) < p_i(x_i). At the first refusal the sequence goes on with
+ * a token drawn from max(0, p_i - q_i) (from p_i where that is zero everywhere), after
+ * counts[b] accepted ones with one drawn from p_counts[b]; counts of 0 only sample. The
+ * draw takes the first index whose running sum is above u times the total. Temperature
+ * 0: p is all on the first index of the maximum (as the greedy loop,
+ * generator.rs:257-265), uniforms do not matter.
+ * accepted [sequences]: how many; emitted [sequences][drafts + 1]: those tokens and the
+ * drawn one, probabilities (nullable, the same shape): the target's p of each; entries
+ * behind them stay as they are. Logits are f32, everything after them 64-bit.
+ * A run that meets what it cannot judge - a target row with a NaN, +infinity or nothing
+ * but -infinity, such a draft row, a token outside the vocabulary, a count outside
+ * 0..drafts, a temperature that is negative or not finite - ends there: the token is -1
+ * with probability 0 and *error is set. Rows behind the end of a run do not matter.
+ * At most 63 drafts, 65535 sequences, a vocabulary of 2^24. workspace as for
+ * rn_attend_shared. */
+int rn_verify_drafts_workspace(int sequences, int drafts, int vocab, size_t* bytes);
+int rn_verify_drafts(int sequences, int drafts, int vocab, const float* target, int64_t target_stride,
+                     const float* draft, int64_t draft_stride, const int32_t* tokens, const int32_t* counts,
+                     const float* temperatures, const float* uniforms, int32_t* accepted, int32_t* emitted,
+                     float* probabilities, void* workspace, size_t workspace_bytes, int32_t* error, void* stream);
 
 /* ---- model API: Model / Session (crates/model/src/model.rs, session.rs) -------- */
 typedef struct {
@@ -424,6 +551,13 @@ int rn_session_truncate(rn_session* session, int length);
 int rn_session_set_cache(rn_session* session, int length, const uint16_t* keys, const uint16_t* values);
 /* Read the first `length` cached positions back (same layout). */
 int rn_session_get_cache(const rn_session* session, int length, uint16_t* keys, uint16_t* values);
+/* The device cache of one layer as the operators over caller-held caches take it
+ * (RN_CACHE_F16, one sequence, every head, the whole capacity; positions from the
+ * session's length on hold nothing): a session that holds a system prompt is the
+ * shared prefix of rn_attend_shared without a copy. The memory is the session's, which
+ * must outlive its use; its pushes and feeds run on rn_session_stream, so work on
+ * another stream has to be ordered after them. */
+int rn_session_layer_cache(const rn_session* session, int layer, rn_cache* out);
 /* Session::push (session.rs:72-148). */
 int rn_session_push(rn_session* session, uint32_t token);
 /* Session::feed (session.rs:56-70): batched prefill on i8 MFMA products. */
@@ -499,6 +633,8 @@ int rn_batch_logits(const rn_batch* batch, float* out);
 /* rn_session_get_cache for one sequence: the first `length` (<= its length)
  * cached positions, [layers][heads][length][head_dim] fp16 bits (host out). */
 int rn_batch_get_cache(const rn_batch* batch, int sequence, int length, uint16_t* keys, uint16_t* values);
+/* rn_session_layer_cache over every sequence of the batch. */
+int rn_batch_layer_cache(const rn_batch* batch, int layer, rn_cache* out);
 int rn_batch_stream(const rn_batch* batch, void** stream);
 
 /* ---- Whistle-style speech path (crates/whistle) -------------------------------- */

@@ -27,6 +27,9 @@ RN_ERR_MEMORY = -5
 FORM_PANEL = 0
 FORM_PLANE = 1
 
+F32, F16 = 0, 1
+CACHE_F16, CACHE_I8 = 0, 1
+
 # Kernel kinds of rn_session_profile_step, in RN_PROFILE_* order.
 PROFILE_KINDS = ("qkv_attention", "out", "gate_up", "down", "logits", "final")
 
@@ -53,6 +56,7 @@ def _load() -> C.CDLL:
 lib = _load()
 
 _i, _f, _p, _u32, _u64, _sz = C.c_int, C.c_float, C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t
+_i64 = C.c_int64
 
 
 class Config(C.Structure):
@@ -94,6 +98,19 @@ class TensorRecord(C.Structure):
 class Choice(C.Structure):
     """rn_choice: the constrained choice and its allowed_statistics (generator.rs:99-194)."""
     _fields_ = [("token", C.c_uint32), ("constrained", C.c_int32), ("probability", C.c_float), ("mass", C.c_float)]
+
+
+class CacheView(C.Structure):
+    """rn_cache."""
+    _fields_ = [("format", C.c_int), ("sequences", C.c_int), ("kv_heads", C.c_int), ("capacity", C.c_int),
+                ("sequence_rows", C.c_int64), ("head_rows", C.c_int64), ("keys", C.c_void_p), ("values", C.c_void_p),
+                ("key_scales", C.c_void_p), ("value_scales", C.c_void_p)]
+
+
+class CacheRows(C.Structure):
+    """rn_cache_rows: rows [sequence][token][head] of 64 values outside a cache, strides in elements."""
+    _fields_ = [("type", C.c_int), ("keys", C.c_void_p), ("values", C.c_void_p), ("sequence_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
 class WhistleConfig(C.Structure):
@@ -182,6 +199,16 @@ SIGNATURES = {
     "rn_reciprocal": (_i, [_p, _p, _i, _p]),
     "rn_zero_centred_norm": (_i, [_p, _p, _i, _i, _p, _p]),
     "rn_attend_heads": (_i, [_p, _p, _p, _p, _i, _i, _i, _p, _p]),
+    "rn_session_layer_cache": (_i, [_p, _i, C.POINTER(CacheView)]),
+    "rn_batch_layer_cache": (_i, [_p, _i, C.POINTER(CacheView)]),
+    "rn_n3_session_layer_cache": (_i, [_p, _i, C.POINTER(CacheView)]),
+    "rn_cache_write": (_i, [C.POINTER(CacheView), C.POINTER(CacheRows), _i, _p, _p, _p, _p]),
+    "rn_cache_read": (_i, [C.POINTER(CacheView), C.POINTER(CacheRows), _i, _p, _p, _p, _p]),
+    "rn_attend_shared_workspace": (_i, [_i, _i, _i, C.POINTER(CacheView), _i, C.POINTER(CacheView), C.POINTER(_sz)]),
+    "rn_attend_shared": (_i, [_p, _i64, _p, _i64, _i, _i, _i, C.POINTER(CacheView), _i, C.POINTER(CacheView), _p, _p,
+                              _f, _i, _p, _sz, _p, _p]),
+    "rn_verify_drafts_workspace": (_i, [_i, _i, _i, C.POINTER(_sz)]),
+    "rn_verify_drafts": (_i, [_i, _i, _i, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _p]),
     "rn_model_create": (_i, [C.POINTER(Config), C.POINTER(WeightsHost), C.POINTER(_p)]),
     "rn_model_create_synthetic": (_i, [C.POINTER(Config), _u64, C.POINTER(_p)]),
     "rn_model_free": (_i, [_p]),
@@ -671,6 +698,100 @@ def attend_heads(q: np.ndarray, K: np.ndarray, V: np.ndarray, lengths: np.ndarra
     return od.download(np.float32, (count, hd))
 
 
+# ---- serving over caller-held caches ---------------------------------------------------
+
+class Cache:
+    """A key/value cache in device memory (rn_cache): 8-bit codes with a scale a row
+    (CACHE_I8) or fp16 rows (CACHE_F16), [sequences][kv_heads][capacity][64]. Its own
+    memory, or with Cache.view the caller's."""
+
+    def __init__(self, format: int, sequences: int, kv_heads: int, capacity: int):
+        rows = int(sequences) * int(kv_heads) * int(capacity)
+        if rows < 1:
+            raise ValueError("sequences, kv_heads and capacity must be positive")
+        size = 64 if format == CACHE_I8 else 128
+        self._memory = [DeviceBuffer(size * rows), DeviceBuffer(size * rows)]
+        if format == CACHE_I8:
+            self._memory += [DeviceBuffer(4 * rows), DeviceBuffer(4 * rows)]
+        p = [m.ptr for m in self._memory] + [None, None]
+        self.struct = CacheView(format, sequences, kv_heads, capacity, kv_heads * capacity, capacity, p[0], p[1], p[2],
+                                p[3])
+
+    @classmethod
+    def view(cls, format: int, sequences: int, kv_heads: int, capacity: int, keys: int, values: int,
+             key_scales: Optional[int] = None, value_scales: Optional[int] = None,
+             sequence_rows: Optional[int] = None, head_rows: Optional[int] = None) -> "Cache":
+        """A cache over the caller's device memory (addresses), which it has to keep;
+        strides in rows, contiguous by default."""
+        self = cls.__new__(cls)
+        self._memory = None
+        heads = capacity if head_rows is None else head_rows
+        self.struct = CacheView(format, sequences, kv_heads, capacity,
+                                kv_heads * heads if sequence_rows is None else sequence_rows, heads, keys, values,
+                                key_scales, value_scales)
+        return self
+
+    @classmethod
+    def _of(cls, entry, owner, layer: int) -> "Cache":
+        """One layer of a session's or batch's own cache; it keeps its owner alive."""
+        self = cls.__new__(cls)
+        self._memory, self.struct = owner, CacheView()
+        check(entry(owner.handle, layer, C.byref(self.struct)))
+        return self
+
+    def write(self, rows: CacheRows, tokens: int, starts: Optional[int] = None, counts: Optional[int] = None,
+              error: Optional[int] = None, stream=None) -> None:
+        """rn_cache_write: `tokens` rows of every sequence and head at starts[b] (device int32 addresses)."""
+        check(lib.rn_cache_write(self.struct, rows, tokens, starts, counts, error, stream))
+
+    def read(self, rows: CacheRows, tokens: int, starts: Optional[int] = None, counts: Optional[int] = None,
+             error: Optional[int] = None, stream=None) -> None:
+        """rn_cache_read: the rows at starts[b] as floats into `rows`."""
+        check(lib.rn_cache_read(self.struct, rows, tokens, starts, counts, error, stream))
+
+
+def attend_shared_workspace(sequences: int, queries: int, heads: int, prefix: Optional[Cache], prefix_length: int,
+                            own: Optional[Cache]) -> int:
+    """Bytes of workspace that attend_shared needs for these arguments."""
+    size = _sz(0)
+    check(lib.rn_attend_shared_workspace(sequences, queries, heads, prefix and prefix.struct, prefix_length,
+                                         own and own.struct, C.byref(size)))
+    return size.value
+
+
+def attend_shared(q: int, out: int, sequences: int, queries: int, heads: int, prefix: Optional[Cache],
+                  prefix_length: int, own: Optional[Cache], lengths: Optional[int] = None,
+                  counts: Optional[int] = None, scale: float = 0.125, window: int = 0,
+                  workspace: Optional[int] = None, workspace_bytes: int = 0, q_stride: Optional[int] = None,
+                  out_stride: Optional[int] = None, error: Optional[int] = None, stream=None) -> None:
+    """rn_attend_shared over device addresses: attention of a batch over one shared
+    prefix and each sequence's own cache. Strides in floats, heads * 64 by default."""
+    row = heads * 64
+    check(lib.rn_attend_shared(q, row if q_stride is None else q_stride, out,
+                               row if out_stride is None else out_stride, sequences, queries, heads,
+                               prefix and prefix.struct, prefix_length, own and own.struct, lengths, counts, scale,
+                               window, workspace, workspace_bytes, error, stream))
+
+
+def verify_drafts_workspace(sequences: int, drafts: int, vocab: int) -> int:
+    """Bytes of workspace that verify_drafts needs for these arguments."""
+    size = _sz(0)
+    check(lib.rn_verify_drafts_workspace(sequences, drafts, vocab, C.byref(size)))
+    return size.value
+
+
+def verify_drafts(sequences: int, drafts: int, vocab: int, target: int, draft: Optional[int], tokens: Optional[int],
+                  counts: Optional[int], temperatures: Optional[int], uniforms: int, accepted: int, emitted: int,
+                  probabilities: Optional[int], workspace: int, workspace_bytes: int,
+                  target_stride: Optional[int] = None, draft_stride: Optional[int] = None,
+                  error: Optional[int] = None, stream=None) -> None:
+    """rn_verify_drafts over device addresses: the accepted run of drafted tokens and the
+    token after it. Strides in floats between rows of logits, `vocab` by default."""
+    check(lib.rn_verify_drafts(sequences, drafts, vocab, target, vocab if target_stride is None else target_stride,
+                               draft, vocab if draft_stride is None else draft_stride, tokens, counts, temperatures,
+                               uniforms, accepted, emitted, probabilities, workspace, workspace_bytes, error, stream))
+
+
 # ---- synthetic inputs ---------------------------------------------------------------
 
 def synth_codes(seed: int, name: str, shape) -> np.ndarray:
@@ -862,6 +983,10 @@ class Session:
         check(lib.rn_session_get_cache(self.handle, length, _ptr(k), _ptr(v)))
         return k.view(np.float16), v.view(np.float16)
 
+    def layer_cache(self, layer: int) -> "Cache":
+        """The device cache of one layer, in place (rn_session_layer_cache)."""
+        return Cache._of(lib.rn_session_layer_cache, self, layer)
+
     def push(self, token: int) -> None:
         check(lib.rn_session_push(self.handle, int(token)))
 
@@ -953,6 +1078,10 @@ class Batch:
         v = np.empty(shape, dtype=np.uint16)
         check(lib.rn_batch_get_cache(self.handle, sequence, length, _ptr(k), _ptr(v)))
         return k.view(np.float16), v.view(np.float16)
+
+    def layer_cache(self, layer: int) -> "Cache":
+        """The device caches of one layer, in place (rn_batch_layer_cache)."""
+        return Cache._of(lib.rn_batch_layer_cache, self, layer)
 
     def stream(self) -> int:
         p = _p()

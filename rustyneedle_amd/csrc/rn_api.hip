@@ -1062,6 +1062,16 @@ int rn_session_get_cache(const rn_session* s, int length, uint16_t* keys, uint16
     return RN_OK;
 }
 
+int rn_session_layer_cache(const rn_session* s, int layer, rn_cache* out) {
+    RN_REQUIRE(s && out, "null argument");
+    const rn_config& c = s->model->cfg;
+    RN_REQUIRE(layer >= 0 && layer < c.layers, "layer %d outside 0..%d", layer, c.layers);
+    const int64_t rows = (int64_t)c.heads * s->capacity;
+    *out = rn_cache{RN_CACHE_F16, 1, c.heads, s->capacity, rows, s->capacity, s->kc + layer * rows * c.head_dim,
+                    s->vc + layer * rows * c.head_dim, nullptr, nullptr};
+    return RN_OK;
+}
+
 // The kernels of one decode step (session.rs:76-148): per layer the norm+QKV
 // product (layer 0 gathers the embedding of state->token first), attention
 // with rotary and the fp16 append, the out product + residual, the
@@ -1924,6 +1934,16 @@ int rn_batch_get_cache(const rn_batch* b, int sequence, int length, uint16_t* ke
     RN_HIP(hipStreamSynchronize(b->stream));
     RN_HIP(hipMemcpy2D(keys, row, b->kc + seq, pitch, row, heads, hipMemcpyDeviceToHost));
     RN_HIP(hipMemcpy2D(values, row, b->vc + seq, pitch, row, heads, hipMemcpyDeviceToHost));
+    return RN_OK;
+}
+
+int rn_batch_layer_cache(const rn_batch* b, int layer, rn_cache* out) {
+    RN_REQUIRE(b && out, "null argument");
+    const rn_config& c = b->model->cfg;
+    RN_REQUIRE(layer >= 0 && layer < c.layers, "layer %d outside 0..%d", layer, c.layers);
+    const int64_t rows = (int64_t)c.heads * b->capacity;
+    *out = rn_cache{RN_CACHE_F16, b->count, c.heads, b->capacity, c.layers * rows, b->capacity,
+                    b->kc + layer * rows * c.head_dim, b->vc + layer * rows * c.head_dim, nullptr, nullptr};
     return RN_OK;
 }
 

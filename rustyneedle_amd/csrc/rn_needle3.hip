@@ -4524,6 +4524,17 @@ int rn_n3_session_cache(rn_n3_session* s, int layer, int8_t* keys, float* key_sc
     return RN_OK;
 }
 
+int rn_n3_session_layer_cache(const rn_n3_session* s, int layer, rn_cache* out) {
+    N3_REQUIRE(s && out, "null argument");
+    N3_REQUIRE(layer >= 0 && layer < (int)s->m->g.num_layers, "layer %d out of range", layer);
+    N3_REQUIRE(std::find(s->m->active.begin(), s->m->active.end(), layer) != s->m->active.end(),
+               "layer %d is not an active layer at this depth", layer);
+    const int KV = (int)s->m->g.num_kv_heads, cap = s->capacity;
+    const N3CacheDev& c = s->caches[(size_t)layer];
+    *out = rn_cache{RN_CACHE_I8, 1, KV, cap, (int64_t)KV * cap, cap, c.keys, c.values, c.key_scales, c.value_scales};
+    return RN_OK;
+}
+
 int rn_n3_session_stream(const rn_n3_session* s, void** stream) {
     N3_REQUIRE(s && stream, "null argument");
     *stream = s->stream;

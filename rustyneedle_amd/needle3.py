@@ -145,7 +145,7 @@ def synthetic_archive(geometry: dict, seed: int = 20261202, bits: Optional[dict]
 
 
 # ---- the device model and session ------------------------------------------------
-from . import Archive, Choice, _ptr, check, lib  # noqa: E402
+from . import Archive, Cache, Choice, _ptr, check, lib  # noqa: E402
 
 _p = __import__("ctypes").c_void_p
 _C = __import__("ctypes")
@@ -275,6 +275,10 @@ class Session:
         vs = np.empty((kv, n), np.float32)
         check(lib.rn_n3_session_cache(self.handle, layer, _ptr(keys), _ptr(ks), _ptr(values), _ptr(vs)))
         return keys, ks, values, vs
+
+    def layer_cache(self, layer: int) -> Cache:
+        """The device cache of an active layer, in place (rn_n3_session_layer_cache)."""
+        return Cache._of(lib.rn_n3_session_layer_cache, self, layer)
 
     def __del__(self):
         try:
