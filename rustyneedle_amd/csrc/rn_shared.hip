@@ -581,11 +581,14 @@ __global__ __launch_bounds__(256, 2) void shared_attend_kernel(const SharedParam
 }
 
 // One wave a row of the output: the shares, each times 2^(its reference - the most).
+// Sixteen lanes hold a row's 64 values, so a wave takes four shares at once; the loads
+// of sixteen are in flight together (one share after the other, a lane a value, waits
+// for every load: 20.8 us against 5.6 for 34 shares of 1920 rows).
 __global__ __launch_bounds__(256) void shared_join_kernel(const SharedParams p) {
     const int id = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
     if (id >= p.rows) return;
     const int heads = p.kv_heads * p.group, token = id / heads;
-    const int b = token / p.queries;
+    const int b = token / p.queries, at = lane % 16 * 4, quarter = lane / 16;
     const Sequence s = sequence_of(p, b);
     float* out = p.out + token * p.out_stride + (id - token * heads) * kCacheWidth;
     if (s.bad) {
@@ -595,22 +598,45 @@ __global__ __launch_bounds__(256) void shared_join_kernel(const SharedParams p) 
     }
     if (token - b * p.queries >= s.count) return;
     const int slots = p.prefix_splits + p.own_splits;
-    float m = -__builtin_inff();
-    for (int k = lane; k < slots; k += 64) {
-        const float2 st = p.stats[(int64_t)k * p.rows + id];
-        if (st.y != 0.0f) m = max_of(m, st.x);
+    v4f o = v4f{0, 0, 0, 0};
+    float l = 0.0f, most = -__builtin_inff();
+    for (int k0 = 0; k0 < slots; k0 += 64) {
+        const int mine = k0 + lane;
+        const float2 st = mine < slots ? p.stats[(int64_t)mine * p.rows + id] : make_float2(0.0f, 0.0f);
+        const float m = max_of(most, wave_max(st.y != 0.0f ? st.x : -__builtin_inff()));
+        if (k0 > 0 && m > most) {
+            const float a = exp2_of(most - m);
+            l *= a;
+            o *= a;
+        }
+        most = m;
+        const float weight = st.y != 0.0f ? exp2_of(st.x - m) : 0.0f;
+        l += weight * st.y;
+        const int here = min(64, slots - k0);
+        for (int k = 0; k < here; k += 16) {
+            v4f v[4];
+            float a[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int slot = k + 4 * u + quarter;
+                a[u] = __shfl(weight, slot & 63);
+                if (slot >= here) a[u] = 0.0f;
+                v[u] = v4f{0, 0, 0, 0};
+                if (a[u] != 0.0f)  // a share without weights holds nothing
+                    v[u] = *reinterpret_cast<const v4f*>(p.parts + ((int64_t)(k0 + slot) * p.rows + id) * kCacheWidth + at);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o += a[u] * v[u];
+        }
     }
-    m = wave_max(m);
-    float o = 0.0f, l = 0.0f;
-    for (int k = 0; k < slots; ++k) {
-        const int64_t r = (int64_t)k * p.rows + id;
-        const float2 st = p.stats[r];
-        if (st.y == 0.0f) continue;
-        const float a = exp2_of(st.x - m);
-        l += a * st.y;
-        o += a * p.parts[r * kCacheWidth + lane];
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) l += __shfl_xor(l, m);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        o[j] += lane_xor<16>(o[j]);
+        o[j] += lane_xor<32>(o[j]);
     }
-    out[lane] = l != 0.0f ? o / l : 0.0f;
+    if (quarter == 0) *reinterpret_cast<v4f*>(out + at) = l != 0.0f ? o / l : v4f{0, 0, 0, 0};
 }
 
 // How a call's rows and keys are dealt to blocks.

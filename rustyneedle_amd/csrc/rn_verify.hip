@@ -10,13 +10,14 @@
 //
 // The border of a draw lies between sums of thousands of weights: in 32 bits about one
 // draw in a hundred would depend on the order of additions. The logits are read in 32
-// bits, and exponentials, sums and the comparison are 64-bit (a 64-bit exponential of
-// 18 operations at the full rate of this chip's vector units), so that the answer is
-// the formula's.
+// bits, and exponentials, sums and the comparison are 64-bit, so that the answer is the
+// formula's. A 64-bit exponential is 15 operations here, at the full rate of this
+// chip's vector units, which keeps the pass over the logits bound by memory.
 //
-// Three launches: every row's maximum and sum by chunks (the only pass over all rows);
-// the accepted run and the chunk sums of the one row that is drawn from; the chunk and
-// index of the draw.
+// First every row's maximum and sum by chunks (the only pass over all rows), then the
+// accepted run and the draw: one block a sequence for vocabularies up to 8192, else
+// the run and the chunk sums of the one row that is drawn from, and the draw's chunk
+// and index in a third launch.
 #include "rn_device.hpp"
 #include "rn_serving.hpp"
 
@@ -40,7 +41,7 @@ struct VerifyParams {
     struct RowPart* parts;   // [sequences][rows a sequence][chunks]
     double2* sums;           // [sequences][chunks]: of the drawn row's rest, and of p
     struct Verdict* verdicts;  // [sequences]
-    int sequences, drafts, vocab, rows, chunks;
+    int sequences, drafts, vocab, rows, chunks, span;
 };
 
 // One chunk of one row: the sum of exp((x - peak) / T), the peak; at temperature 0 the
@@ -56,7 +57,7 @@ struct RowPart {
 
 // What the draw needs to know of its sequence.
 struct Verdict {
-    double p_scale, q_scale;  // 1 / total of the target's and the draft's row
+    double p_scale, ratio;  // 1 / sum of the target's row; sum of it over that of the draft's
     float p_peak, q_peak;
     int32_t at;       // accepted tokens; the row of the draw
     int32_t refused;  // the rest of row `at` is drawn from, not all of it
@@ -64,40 +65,84 @@ struct Verdict {
     int32_t spare;
 };
 
-// exp(x) for x <= 0, relative error below 1e-13: x = n ln2 + r, |r| <= ln2 / 2, the
-// series of exp(r) to r^10 (the next term is at most 2.2e-13), times 2^n.
-__device__ __forceinline__ double exp64(double x) {
-    const double n = __builtin_rint(x * 1.4426950408889634);
-    double r = __builtin_fma(n, -0x1.62e42fefa39efp-1, x);
-    r = __builtin_fma(n, -0x1.abc9e3b39803fp-56, r);
-    double y = 1.0 / 3628800.0;
-    y = __builtin_fma(y, r, 1.0 / 362880.0);
-    y = __builtin_fma(y, r, 1.0 / 40320.0);
-    y = __builtin_fma(y, r, 1.0 / 5040.0);
-    y = __builtin_fma(y, r, 1.0 / 720.0);
-    y = __builtin_fma(y, r, 1.0 / 120.0);
-    y = __builtin_fma(y, r, 1.0 / 24.0);
-    y = __builtin_fma(y, r, 1.0 / 6.0);
-    y = __builtin_fma(y, r, 0.5);
-    y = __builtin_fma(y, r, 1.0);
-    y = __builtin_fma(y, r, 1.0);
-    return __builtin_ldexp(y, (int)(n < -2000.0 ? -2000.0 : n));
+// 2^y for -1000 <= y <= 0, relative error below 1.1e-12: y = n + r, |r| <= 1/2, 2^r by
+// its interpolation of degree 8 at the Chebyshev nodes of that interval (exact at 0),
+// n added to the exponent. n comes from the low bits of y + 1.5 2^52.
+__device__ __forceinline__ double exp2_64(double y) {
+    const double t = y + 0x1.8p+52, r = y - (t - 0x1.8p+52);
+    double p = 0x1.63d1363a681b4p-20;
+    p = __builtin_fma(p, r, 0x1.00dc4a5344ef5p-16);
+    p = __builtin_fma(p, r, 0x1.4308ac85a69f8p-13);
+    p = __builtin_fma(p, r, 0x1.5d8745a728209p-10);
+    p = __builtin_fma(p, r, 0x1.3b2ab7181b77dp-7);
+    p = __builtin_fma(p, r, 0x1.c6b08dd6fd236p-5);
+    p = __builtin_fma(p, r, 0x1.ebfbdff823cedp-3);
+    p = __builtin_fma(p, r, 0x1.62e42fef84cf0p-1);
+    p = __builtin_fma(p, r, 1.0);
+    const uint64_t bits = (uint64_t)__double_as_longlong(p);
+    const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)(uint64_t)__double_as_longlong(t) << 20);
+    return __longlong_as_double((long long)(((uint64_t)hi << 32) | (uint32_t)bits));
 }
 
-// exp((x - peak) / T), 0 for a masked logit; `warm` = 1 / T.
-__device__ __forceinline__ double weight(float x, float peak, double warm) {
-    return x > -__builtin_inff() ? exp64(((double)x - (double)peak) * warm) : 0.0;
+// exp((x - peak) / T) with warm = log2(e) / T. What is less than 2^-1000, a masked
+// logit among it, comes out as 2^-1000, which no sum of a row notices (its peak's is
+// 1); a weight counts from kLeast on.
+__device__ __forceinline__ double weight(float x, double peak, double warm) {
+    return exp2_64(__builtin_fmax(((double)x - peak) * warm, -1000.0));
+}
+constexpr double kLeast = 0x1p-990;  // of one index; 2^24 masked ones sum up to less than kMost
+constexpr double kMost = 0x1p-970;
+__device__ __forceinline__ double likely(float x, double peak, double warm) {
+    const double w = weight(x, peak, warm);
+    return w < kLeast ? 0.0 : w;
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int m) {
-    const uint64_t u = (uint64_t)__double_as_longlong(v);
-    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, m), hi = (uint32_t)__shfl_xor((int)(uint32_t)(u >> 32), m);
+__device__ __forceinline__ double of_halves(uint32_t lo, uint32_t hi) {
     return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-    for (int m = 1; m < 64; m <<= 1) v += shfl_xor_f64(v, m);
-    return v;
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return of_halves((uint32_t)dpp_move<CTRL>((int)(uint32_t)u), (uint32_t)dpp_move<CTRL>((int)(uint32_t)(u >> 32)));
 }
+// The sum over each run of 8 lanes, in all of them.
+__device__ __forceinline__ double row8_sum(double v) {
+    v += dpp_f64<0xb1>(v);
+    v += dpp_f64<0x4e>(v);
+    return v + dpp_f64<0x141>(v);
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    return __longlong_as_double((long long)lane_u64((uint64_t)__double_as_longlong(v), lane));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = row8_sum(v);
+    v += dpp_f64<0x140>(v);
+    return (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
+}
+__device__ __forceinline__ float row8_max(float v) {
+    v = fmaxf(v, __int_as_float(dpp_move<0xb1>(__float_as_int(v))));
+    v = fmaxf(v, __int_as_float(dpp_move<0x4e>(__float_as_int(v))));
+    return fmaxf(v, __int_as_float(dpp_move<0x141>(__float_as_int(v))));
+}
+// The sum of this lane's and all lower lanes' values: in each row of 16 lanes by row
+// shifts (a lane without a source adds 0), then the rows below.
+template <int SHIFT>
+__device__ __forceinline__ double row_shift_f64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return of_halves((uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x110 + SHIFT, 0xf, 0xf, true),
+                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), 0x110 + SHIFT, 0xf, 0xf, true));
+}
+__device__ __forceinline__ double wave_scan(double v) {
+    v += row_shift_f64<1>(v);
+    v += row_shift_f64<2>(v);
+    v += row_shift_f64<4>(v);
+    v += row_shift_f64<8>(v);
+    const double a = lane_f64(v, 15), b = a + lane_f64(v, 31), c = b + lane_f64(v, 47);
+    const int row = threadIdx.x % 64 / 16;
+    return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
+}
+
+constexpr double kLog2e = 1.4426950408889634;
 
 // Four consecutive logits of a row at i (-infinity past its end); rows need no more
 // than the alignment of a float.
@@ -157,12 +202,15 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
     double sum = 0.0;
     uint64_t key = 0;
     if (temperature > 0.0f) {
-        const double warm = 1.0 / (double)temperature;
+        // a chunk of masked logits has no sum; elsewhere their 2^-1000 do not matter
+        if (peak > -__builtin_inff()) {
+            const double warm = kLog2e / (double)temperature;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+            for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sum += weight(x[e][c], peak, warm);
-        sum = wave_sum(sum);
+                for (int c = 0; c < 4; ++c) sum += weight(x[e][c], (double)peak, warm);
+            sum = wave_sum(sum);
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -196,38 +244,45 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
 
 constexpr int kMaxDrafts = 63;  // a lane each, and one for the draw
 
-// The weights of the draw at four logits: what is left of p, and p.
+// The weights of the draw at four logits, times the sum of the target's row: what is
+// left of p, and p.
 struct Draw {
-    double warm, p_scale, q_scale;
-    float p_peak, q_peak;
+    double warm, p_peak, q_peak, ratio;
     const float* p_row;
     const float* q_row;  // null: nothing is taken off but `token`
     int token;           // taken off p where there are no draft logits; -1: none
     int vocab;
 
-    __device__ __forceinline__ void at(int i, double* rest, double* all) const {
-        float x[4], y[4];
+    __device__ __forceinline__ void load(int i, float* x, float* y) const {
         load_logits(p_row, i, vocab, x);
         if (q_row) load_logits(q_row, i, vocab, y);
+    }
+    __device__ __forceinline__ void at(int i, double* rest, double* all) const {
+        float x[4], y[4];
+        load(i, x, y);
+        of(i, x, y, rest, all);
+    }
+    __device__ __forceinline__ void of(int i, const float* x, const float* y, double* rest, double* all) const {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const double w = weight(x[c], p_peak, warm) * p_scale;
-            double left = w;
-            if (q_row) left = w - weight(y[c], q_peak, warm) * q_scale;
-            if (i + c == token) left = 0.0;
-            all[c] = w;
-            rest[c] = left > 0.0 ? left : 0.0;
+        for (int c = 0; c < 4; ++c) rest[c] = all[c] = weight(x[c], p_peak, warm);
+        if (q_row) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                rest[c] = __builtin_fmax(__builtin_fma(-weight(y[c], q_peak, warm), ratio, all[c]), 0.0);
+        } else if (token >= 0) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (i + c == token) rest[c] = 0.0;
         }
     }
 };
 
 __device__ __forceinline__ Draw draw_of(const VerifyParams& p, int b, const Verdict& v, float temperature) {
     Draw d;
-    d.warm = 1.0 / (double)temperature;
-    d.p_scale = v.p_scale;
-    d.q_scale = v.q_scale;
-    d.p_peak = v.p_peak;
-    d.q_peak = v.q_peak;
+    d.warm = kLog2e / (double)temperature;
+    d.p_peak = (double)v.p_peak;
+    d.q_peak = (double)v.q_peak;
+    d.ratio = v.ratio;
     d.p_row = row_of(p, b, v.at);
     d.q_row = v.refused && p.draft ? row_of(p, b, p.drafts + 1 + v.at) : nullptr;
     d.token = v.refused && !p.draft ? p.tokens[b * p.drafts + v.at] : -1;
@@ -235,74 +290,96 @@ __device__ __forceinline__ Draw draw_of(const VerifyParams& p, int b, const Verd
     return d;
 }
 
-// The accepted run of a sequence (every block of it finds the same), and the sums of
-// this block's chunk of the row that is drawn from.
-template <int E>
-__global__ __launch_bounds__(kThreads) void verify_run_kernel(const VerifyParams p) {
-    const int chunk = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t % 64, wave = t / 64;
-    __shared__ double totals[2 * kMaxDrafts + 1];
-    __shared__ float peaks[2 * kMaxDrafts + 1];
-    __shared__ int firsts[2 * kMaxDrafts + 1];  // greedy: the first largest index; -1: the row is bad
-    __shared__ Verdict verdict;
-    __shared__ double2 sums[4];
-    float temperature;
+struct Rows {
+    double totals[2 * kMaxDrafts + 1], inverse[2 * kMaxDrafts + 1];  // sum of the row's weights, 1 / it
+    float peaks[2 * kMaxDrafts + 1];
+    int firsts[2 * kMaxDrafts + 1];  // greedy: the first largest index; -1: the row is bad
+    Verdict verdict;
+};
+
+// The accepted run of a sequence, by a whole block; with `tell` it is written down.
+template <int THREADS>
+__device__ __forceinline__ Verdict judge(const VerifyParams& p, int b, float& temperature, Rows& rows, bool tell) {
+    const int t = threadIdx.x, lane = t % 64, wave = t / 64;
+    // what lane i needs of drafted token i, asked for before anything is waited for
+    int token = -1;
+    float u = 0.0f, x = 0.0f, y = 0.0f;
+    const bool mine = wave == 0 && lane < p.drafts;
+    if (mine) {
+        token = p.tokens[b * p.drafts + lane];
+        u = p.uniforms[b * (p.drafts + 1) + lane];
+    }
     const int count = count_of(p, b, temperature);
     const bool greedy = !(temperature > 0.0f);
-    const double warm = greedy ? 0.0 : 1.0 / (double)temperature;
-    // ---- every row's total, a wave a row
-    for (int r = wave; r < p.rows; r += 4) {
+    if (mine && token >= 0 && token < p.vocab) {
+        x = row_of(p, b, lane)[token];
+        if (p.draft) y = row_of(p, b, p.drafts + 1 + lane)[token];
+    }
+    const double warm = greedy ? 0.0 : kLog2e / (double)temperature;
+    // ---- every row's total, eight lanes a row
+    for (int r = t / 8; r < p.rows; r += THREADS / 8) {
         if (r > p.drafts ? r - p.drafts - 1 >= count : r > count) continue;
         const RowPart* parts = p.parts + ((int64_t)b * p.rows + r) * p.chunks;
         float peak = -__builtin_inff();
-        bool bad = false;
-        uint64_t key = 0;
-        for (int c = lane; c < p.chunks; c += 64) {
-            peak = fmaxf(peak, parts[c].peak);
-            bad = bad || parts[c].bad;
-            if (greedy) key = parts[c].key > key ? parts[c].key : key;
-        }
-        peak = wave_max(peak);
-        bad = __any(bad) || !(peak > -__builtin_inff());
         double total = 0.0;
-        if (greedy) {
-            key = wave_max_u64(key);
-        } else if (!bad) {
-            for (int c = lane; c < p.chunks; c += 64) total += parts[c].sum * weight(parts[c].peak, peak, warm);
-            total = wave_sum(total);
+        int bad = 0;
+        uint64_t key = 0;
+#pragma unroll 2
+        for (int c = lane % 8; c < p.chunks; c += 8) {
+            const RowPart part = parts[c];
+            bad |= part.bad;
+            if (greedy) {
+                key = part.key > key ? part.key : key;
+                peak = fmaxf(peak, part.peak);
+            } else if (part.peak > peak) {
+                total = total * likely(peak, part.peak, warm) + part.sum;
+                peak = part.peak;
+            } else if (part.peak > -__builtin_inff()) {
+                total += part.sum * likely(part.peak, peak, warm);
+            }
         }
-        if (lane == 0) {
-            totals[r] = total;
-            peaks[r] = peak;
-            firsts[r] = bad ? -1 : greedy ? (int)argmax_index(key) : 0;
+        const float most = row8_max(peak);
+        bad |= dpp_move<0xb1>(bad);
+        bad |= dpp_move<0x4e>(bad);
+        bad |= dpp_move<0x141>(bad);
+        if (greedy) {
+            key = max_with_dpp_u64<0xb1>(key);
+            key = max_with_dpp_u64<0x4e>(key);
+            key = max_with_dpp_u64<0x141>(key);
+        } else {
+            total = row8_sum(peak > -__builtin_inff() ? total * likely(peak, most, warm) : 0.0);
+        }
+        if (lane % 8 == 0) {
+            rows.totals[r] = total;
+            rows.inverse[r] = 1.0 / total;
+            rows.peaks[r] = most;
+            rows.firsts[r] = bad || !(most > -__builtin_inff()) ? -1 : greedy ? (int)argmax_index(key) : 0;
         }
     }
     __syncthreads();
     // ---- the accepted run: lane i judges drafted token i, lane `count` the draw's row
     if (wave == 0) {
         int state = 0;  // 0 accepted, 1 the run ends here, 2 it cannot be judged
-        int token = -1;
         double chance = 0.0;  // of the drafted token, under the target
         if (count < 0) {
             state = 2;
         } else if (lane <= count) {
-            if (firsts[lane] < 0) {
+            if (rows.firsts[lane] < 0) {
                 state = 2;
             } else if (lane == count) {
                 state = 1;
             } else {
-                token = p.tokens[b * p.drafts + lane];
                 const int dr = p.drafts + 1 + lane;
-                if (token < 0 || token >= p.vocab || (p.draft && firsts[dr] < 0)) {
+                if (token < 0 || token >= p.vocab || (p.draft && rows.firsts[dr] < 0)) {
                     state = 2;
                 } else if (greedy) {
-                    chance = token == firsts[lane] ? 1.0 : 0.0;
-                    state = token == firsts[lane] ? 0 : 1;
+                    chance = token == rows.firsts[lane] ? 1.0 : 0.0;
+                    state = token == rows.firsts[lane] ? 0 : 1;
                 } else {
-                    const float x = row_of(p, b, lane)[token];
-                    chance = weight(x, peaks[lane], warm) / totals[lane];
+                    chance = likely(x, rows.peaks[lane], warm) * rows.inverse[lane];
                     double q = 1.0;
-                    if (p.draft) q = weight(row_of(p, b, dr)[token], peaks[dr], warm) / totals[dr];
-                    state = (double)p.uniforms[b * (p.drafts + 1) + lane] * q < chance ? 0 : 1;
+                    if (p.draft) q = likely(y, rows.peaks[dr], warm) * rows.inverse[dr];
+                    state = (double)u * q < chance ? 0 : 1;
                 }
             }
         } else {
@@ -311,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void verify_run_kernel(const VerifyParams
         const uint64_t ends = __ballot(state != 0);
         const int at = __builtin_ctzll(ends);  // count <= 63: some lane ends the run
         const int end = __shfl(state, at);
-        if (chunk == 0) {
+        if (tell) {
             if (lane < at) {
                 p.emitted[b * (p.drafts + 1) + lane] = token;
                 if (p.probabilities) p.probabilities[b * (p.drafts + 1) + lane] = (float)chance;
@@ -323,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void verify_run_kernel(const VerifyParams
                     if (p.probabilities) p.probabilities[b * (p.drafts + 1) + at] = 0.0f;
                     if (p.error) *p.error = RN_ERR_ARGUMENT;
                 } else if (greedy) {
-                    p.emitted[b * (p.drafts + 1) + at] = firsts[at];
+                    p.emitted[b * (p.drafts + 1) + at] = rows.firsts[at];
                     if (p.probabilities) p.probabilities[b * (p.drafts + 1) + at] = 1.0f;
                 }
             }
@@ -332,125 +409,198 @@ __global__ __launch_bounds__(kThreads) void verify_run_kernel(const VerifyParams
             Verdict v{};
             v.at = at;
             v.refused = at < count;
-            v.choice = end == 2 ? -2 : greedy ? firsts[at] : -1;
+            v.choice = end == 2 ? -2 : greedy ? rows.firsts[at] : -1;
             if (v.choice == -1) {
-                v.p_scale = 1.0 / totals[at];
-                v.p_peak = peaks[at];
+                v.p_scale = rows.inverse[at];
+                v.p_peak = rows.peaks[at];
                 if (v.refused && p.draft) {
-                    v.q_scale = 1.0 / totals[p.drafts + 1 + at];
-                    v.q_peak = peaks[p.drafts + 1 + at];
+                    v.ratio = rows.totals[at] / rows.totals[p.drafts + 1 + at];  // 1 for equal rows
+                    v.q_peak = rows.peaks[p.drafts + 1 + at];
                 }
             }
-            verdict = v;
-            if (chunk == 0) p.verdicts[b] = v;
+            rows.verdict = v;
         }
     }
     __syncthreads();
-    const Verdict v = verdict;
-    if (v.choice != -1) return;
-    const Draw d = draw_of(p, b, v, temperature);
-    double rest = 0.0, all = 0.0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        double r4[4], a4[4];
-        d.at((chunk * E + e) * kThreads * 4 + t * 4, r4, a4);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            rest += r4[c];
-            all += a4[c];
-        }
-    }
-    rest = wave_sum(rest);
-    all = wave_sum(all);
-    if (lane == 0) sums[wave] = make_double2(rest, all);
-    __syncthreads();
-    if (t == 0)
-        p.sums[(int64_t)b * p.chunks + chunk] = make_double2(((sums[0].x + sums[1].x) + sums[2].x) + sums[3].x,
-                                                             ((sums[0].y + sums[1].y) + sums[2].y) + sums[3].y);
+    return rows.verdict;
 }
 
-// The draw: the chunk whose running sum passes u times the total, and in it the index.
-template <int E>
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyParams p) {
-    const int b = blockIdx.x, t = threadIdx.x, lane = t % 64, wave = t / 64;
-    const Verdict v = p.verdicts[b];
-    if (v.choice != -1) return;
-    const float temperature = p.temperatures ? p.temperatures[b] : 1.0f;
-    const Draw d = draw_of(p, b, v, temperature);
-    __shared__ double before[4];
-    __shared__ int found[4], last[4];
-    const double2* sums = p.sums + (int64_t)b * p.chunks;
-    // every thread walks the chunks in order
-    double total = 0.0;
-    for (int c = 0; c < p.chunks; ++c) total += sums[c].x;
-    const bool whole = !(total > 0.0);  // nothing is left of p: all of it
-    if (whole) {
-        total = 0.0;
-        for (int c = 0; c < p.chunks; ++c) total += sums[c].y;
-    }
-    const double border = (double)p.uniforms[b * (p.drafts + 1) + p.drafts] * total;
-    double running = 0.0, base = 0.0;
-    int chunk = 0;
-    for (int c = 0; c < p.chunks; ++c) {
-        const double s = whole ? sums[c].y : sums[c].x;
-        if (s > 0.0) {
-            chunk = c;
-            base = running;
-            if (running + s > border) break;
+// The draw among this block's 4 E THREADS consecutive weights w from `first` on (each
+// thread its run of 4 E, their sum `mine`, `upto` that of the wave's lanes up to it,
+// `sums` that of every wave): the first index whose running sum, `base` before them,
+// is above `border`; past the end, by a rounding or by a uniform of 1, the last with a
+// weight. The one thread that holds it writes it down, with its weight under the target.
+template <int THREADS, int E>
+__device__ __forceinline__ void pick(const VerifyParams& p, int b, const Verdict& v, const double (&w)[E][4],
+                                     const double (&all)[E][4], double mine, double upto, const double* sums,
+                                     double base, double border, int first) {
+    const int t = threadIdx.x, lane = t % 64, wave = t / 64;
+    // every wave finds the wave, that one the lane, that one the index
+    int chosen = -1;
+    double below = base, mark = base;
+    for (int k = 0; k < THREADS / 64; ++k) {
+        const double s = sums[k];
+        if (s > kMost) {
+            chosen = k;
+            mark = below;
+            if (below + s > border) break;
         }
-        running += s;
+        below += s;
     }
-    // this thread's run of 4 E indices in order
-    double w[E][4], mine = 0.0;
-    const int first = (chunk * kThreads + t) * E * 4;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        double rest[4], all[4];
-        d.at(first + 4 * e, rest, all);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            w[e][c] = whole ? all[c] : rest[c];
-            mine += w[e][c];
-        }
-    }
-    double upto = mine;  // inclusive over the wave's lanes
-    for (int m = 1; m < 64; m <<= 1) {
-        const uint64_t u = (uint64_t)__double_as_longlong(upto);
-        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, m), hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), m);
-        if (lane >= m) upto += __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
-    }
-    if (lane == 63) before[wave] = upto;
-    __syncthreads();
-    double sum = base + (upto - mine);
-    for (int k = 0; k < wave; ++k) sum += before[k];
-    int hit = 0x7fffffff, most = -1;
+    if (wave != chosen) return;
+    const uint64_t over = __ballot(mine > kMost && mark + upto > border), some = __ballot(mine > kMost);
+    if (some == 0 || lane != (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some))) return;
+    double sum = mark + (upto - mine), chance = 0.0;
+    int token = -1;
+    bool done = false;
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-            if (w[e][c] > 0.0) {
+            if (w[e][c] > kLeast && !done) {
                 sum += w[e][c];
-                const int i = first + 4 * e + c;
-                if (sum > border && hit == 0x7fffffff) hit = i;
-                most = i;
+                token = first + 4 * e + c;
+                chance = all[e][c];
+                done = sum > border;
             }
-    for (int m = 1; m < 64; m <<= 1) {
-        hit = min(hit, __shfl_xor(hit, m));
-        most = max(most, __shfl_xor(most, m));
+    const int at = b * (p.drafts + 1) + v.at;
+    p.emitted[at] = token;
+    if (p.probabilities) p.probabilities[at] = (float)(chance * v.p_scale);
+}
+
+constexpr int kWide = 1024;  // threads of a block that holds a whole row
+
+// The accepted run and the draw of a sequence whose vocabulary one block holds.
+template <int E>
+__global__ __launch_bounds__(kWide) void verify_finish_kernel(const VerifyParams p) {
+    const int b = blockIdx.x, t = threadIdx.x, lane = t % 64, wave = t / 64;
+    __shared__ Rows rows;
+    __shared__ double rests[kWide / 64], wholes[kWide / 64];
+    float temperature;
+    const float u = p.uniforms[b * (p.drafts + 1) + p.drafts];
+    const Verdict v = judge<kWide>(p, b, temperature, rows, true);
+    if (v.choice != -1) return;
+    const Draw d = draw_of(p, b, v, temperature);
+    double w[E][4], a[E][4], mine = 0.0;
+    const int first = t * E * 4;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        d.at(first + 4 * e, w[e], a[e]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mine += w[e][c];
     }
-    if (lane == 0) {
-        found[wave] = hit;
-        last[wave] = most;
+    double upto = wave_scan(mine);
+    if (lane == 63) rests[wave] = upto;
+    __syncthreads();
+    double total = 0.0;
+    double* sums = rests;
+    for (int k = 0; k < kWide / 64; ++k) total += rests[k];
+    if (!(total > kMost)) {  // nothing is left of p: all of it
+        mine = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                w[e][c] = a[e][c];
+                mine += a[e][c];
+            }
+        upto = wave_scan(mine);
+        if (lane == 63) wholes[wave] = upto;
+        __syncthreads();
+        total = 0.0;
+        for (int k = 0; k < kWide / 64; ++k) total += wholes[k];
+        sums = wholes;
+    }
+    pick<kWide, E>(p, b, v, w, a, mine, upto, sums, 0.0, (double)u * total, first);
+}
+
+constexpr int kSpan = 8;  // most chunks a block
+
+// The accepted run of a sequence (every block of it finds the same), and the sums of
+// this block's chunks, four logits a thread, of the row that is drawn from. Few blocks
+// of several chunks, the next one's logits asked for in time: judged in a launch of its
+// own, with a block a chunk after it, the two took 17.7 us for 64 sequences of 65536.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void verify_run_kernel(const VerifyParams p) {
+    const int b = blockIdx.y, t = threadIdx.x, lane = t % 64, wave = t / 64;
+    const int c0 = blockIdx.x * p.span, c1 = min(c0 + p.span, p.chunks);
+    __shared__ Rows rows;
+    __shared__ double2 sums[kSpan][THREADS / 64];
+    float temperature;
+    const Verdict v = judge<THREADS>(p, b, temperature, rows, c0 == 0);
+    if (c0 == 0 && t == 0) p.verdicts[b] = v;
+    if (v.choice != -1) return;
+    const Draw d = draw_of(p, b, v, temperature);
+    float x[4], y[4];
+    d.load((c0 * THREADS + t) * 4, x, y);
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) {
+        double r4[4], a4[4];
+        const float x0[4] = {x[0], x[1], x[2], x[3]}, y0[4] = {y[0], y[1], y[2], y[3]};
+        if (c + 1 < c1) d.load(((c + 1) * THREADS + t) * 4, x, y);
+        d.of((c * THREADS + t) * 4, x0, y0, r4, a4);
+        const double rest = wave_sum((r4[0] + r4[1]) + (r4[2] + r4[3])), all = wave_sum((a4[0] + a4[1]) + (a4[2] + a4[3]));
+        if (lane == 0) sums[c - c0][wave] = make_double2(rest, all);
     }
     __syncthreads();
-    if (t == 0) {
-        hit = min(min(found[0], found[1]), min(found[2], found[3]));
-        // past the end by a rounding, or by a uniform of 1: the last index with a weight
-        if (hit == 0x7fffffff) hit = max(max(last[0], last[1]), max(last[2], last[3]));
-        const int at = b * (p.drafts + 1) + v.at;
-        p.emitted[at] = hit;
-        if (p.probabilities) p.probabilities[at] = (float)(weight(d.p_row[hit], v.p_peak, d.warm) * v.p_scale);
+    if (t < c1 - c0) {
+        double2 s = sums[t][0];
+        for (int k = 1; k < THREADS / 64; ++k) {
+            s.x += sums[t][k].x;
+            s.y += sums[t][k].y;
+        }
+        p.sums[(int64_t)b * p.chunks + c0 + t] = s;
     }
+}
+
+// The draw: the chunk whose running sum passes u times the total, and in it the index.
+// Every wave finds the chunk by itself, a lane a chunk.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void verify_draw_kernel(const VerifyParams p) {
+    const int b = blockIdx.x, t = threadIdx.x, lane = t % 64, wave = t / 64;
+    const float u = p.uniforms[b * (p.drafts + 1) + p.drafts];
+    const float temperature = p.temperatures ? p.temperatures[b] : 1.0f;
+    const double2* sums = p.sums + (int64_t)b * p.chunks;
+    const Verdict v = p.verdicts[b];
+    if (v.choice != -1) return;
+    __shared__ double waves[THREADS / 64];
+    double rest = 0.0, all = 0.0;
+    for (int c = lane; c < p.chunks; c += 64) {
+        const double2 s = sums[c];
+        rest += s.x;
+        all += s.y;
+    }
+    rest = wave_sum(rest);
+    const bool whole = !(rest > kMost);  // nothing is left of p: all of it
+    const double border = (double)u * (whole ? wave_sum(all) : rest);
+    double base = 0.0, running = 0.0;
+    int chunk = 0;
+    for (int c0 = 0; c0 < p.chunks; c0 += 64) {
+        double s = 0.0;
+        if (c0 + lane < p.chunks) s = whole ? sums[c0 + lane].y : sums[c0 + lane].x;
+        const double upto = running + wave_scan(s);
+        const uint64_t over = __ballot(s > kMost && upto > border), some = __ballot(s > kMost);
+        // the first chunk that passes the border, or the last with a weight so far
+        const int at = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+        if (at >= 0) {
+            chunk = c0 + at;
+            base = lane_f64(upto, at) - lane_f64(s, at);
+        }
+        if (over) break;
+        running = lane_f64(upto, 63);
+    }
+    const Draw d = draw_of(p, b, v, temperature);
+    double w[1][4], a[1][4];
+    const int first = (chunk * THREADS + t) * 4;
+    d.at(first, w[0], a[0]);
+    if (whole) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[0][c] = a[0][c];
+    }
+    const double mine = (w[0][0] + w[0][1]) + (w[0][2] + w[0][3]), upto = wave_scan(mine);
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    pick<THREADS, 1>(p, b, v, w, a, mine, upto, waves, base, border, first);
 }
 
 struct VerifyPlan {
@@ -537,16 +687,20 @@ int rn_verify_drafts(int sequences, int drafts, int vocab, const float* target, 
     p.vocab = vocab;
     p.rows = draft ? n.rows : drafts + 1;
     p.chunks = n.chunks;
+    // as many chunks a block as leave a block a CU: each block judges the run again
+    const int64_t span = (int64_t)sequences * n.chunks / 256;
+    p.span = span < 1 ? 1 : span > kSpan ? kSpan : (int)span;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 rows(n.chunks, p.rows, sequences), run(n.chunks, sequences), draw(sequences), block(kThreads);
-    if (n.each == 4) {
-        rn_launch(verify_rows_kernel<4>, rows, block, 0, s, p);
-        rn_launch(verify_run_kernel<4>, run, block, 0, s, p);
-        rn_launch(verify_draw_kernel<4>, draw, block, 0, s, p);
+    const dim3 rows(n.chunks, p.rows, sequences), run((n.chunks + p.span - 1) / p.span, sequences), draw(sequences), block(kThreads);
+    rn_launch(n.each == 4 ? verify_rows_kernel<4> : verify_rows_kernel<1>, rows, block, 0, s, p);
+    if (vocab <= kWide * 8) {
+        rn_launch(vocab <= kWide * 4 ? verify_finish_kernel<1> : verify_finish_kernel<2>, draw, dim3(kWide), 0, s, p);
+    } else if (n.each == 4) {
+        rn_launch(verify_run_kernel<4 * kThreads>, run, dim3(4 * kThreads), 0, s, p);
+        rn_launch(verify_draw_kernel<4 * kThreads>, draw, dim3(4 * kThreads), 0, s, p);
     } else {
-        rn_launch(verify_rows_kernel<1>, rows, block, 0, s, p);
-        rn_launch(verify_run_kernel<1>, run, block, 0, s, p);
-        rn_launch(verify_draw_kernel<1>, draw, block, 0, s, p);
+        rn_launch(verify_run_kernel<kThreads>, run, block, 0, s, p);
+        rn_launch(verify_draw_kernel<kThreads>, draw, block, 0, s, p);
     }
     SV_HIP(hipGetLastError());
     return RN_OK;
