@@ -447,15 +447,19 @@ int rn_cache_read(const rn_cache* cache, const rn_cache_rows* rows, int tokens, 
  * scale times q . k, out = sum softmax(score) v; a query that sees nothing gives
  * zeros. Rows past counts[b] stay as they are. Positions a query does not see never
  * reach it, whatever they hold; a NaN or infinity that it sees makes its output so.
- * scale must be positive and finite.
+ * scale must be positive and finite. Value rows' scales are positive, as rn_cache_write
+ * leaves them: below 2^-100 they count as 0, negative and infinite ones and NaN make the
+ * output of the queries that see them NaN, and those a query sees should lie within
+ * 2^116 of one another (zeros aside: below 2^16), or small weights are lost.
  * Products and sums are f32 (queries and weights enter the matrix instructions as
  * pairs of fp16 numbers, 22 bits; relative error about 1e-6); the result depends on
- * the shapes and lengths only and repeats bit for bit.
+ * the shapes, lengths, counts and window only and repeats bit for bit.
  * A sequence with lengths[b] outside 0..capacity or counts[b] outside 0..queries gets
  * NaN in all its rows. workspace: workspace_bytes of device memory aligned to 256
- * bytes, at least what rn_attend_shared_workspace says for the same arguments; its
- * contents need not be kept, and calls that may run at the same time (two streams, two
- * graphs) need one each. At most 2^20 rows sequences * queries * heads. */
+ * bytes, at least what rn_attend_shared_workspace says for the same arguments (0 where
+ * the work is small, and it may be null then); its contents need not be kept, and calls
+ * that may run at the same time (two streams, two graphs) need one each. At most 2^20
+ * rows sequences * queries * heads. */
 int rn_attend_shared_workspace(int sequences, int queries, int heads, const rn_cache* prefix, int prefix_length,
                                const rn_cache* own, size_t* bytes);
 int rn_attend_shared(const float* q, int64_t q_stride, float* out, int64_t out_stride, int sequences, int queries,

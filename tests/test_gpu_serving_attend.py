@@ -7,17 +7,18 @@ B (2 ds + dw + dn):
       of it together, or 2^-24 of the row's peak), 64 products are added in f32 (at
       most 130 roundings of 2^-24), the scale and the exponent's argument are rounded
       to 2^-24 of values up to A log2(e), 4 times: A (2^-20 + 134 x 1.5 x 2^-24) and
-      64 x 2^-24 of scale x peak x the largest |k|;
+      64 x 2^-24 of scale x peak x the largest |k|; the logarithm L of the value's scale
+      is rounded to 2^-23 and enters 4 rounded sums: 6 ln 2 |L| 2^-24;
       it enters a weight and the total: twice;
-  dw  a weight's: the exponential (2^-22), the value's scale (2^-24), two fp16 parts
-      (2^-20);
+  dw  a weight's: the exponential (2^-22), the inverse of the value's scale (2^-23), two
+      fp16 parts (2^-20);
   dn  f32 sums of n weights and of n products in some order, and the joining of the
       shares: 2 (n + 64) 2^-24.
-And by the floor of the weights: times 2^14 and over the bound of the value scales they
-are fp16 pairs, whose low part is cut at the step 2^-24 of the smallest numbers, so each
-may be off by 2^-38 of the largest one; times |v| over that bound (fp16: |v|; 8 bits:
-|code| times the bound, which is up to twice the largest scale, and a row of 64 random
-codes holds one above 63, so at most 4 max |v|), over a total of at least 1:
+And by the floor of the weights: weight x value scale, times 2^14 over the largest such
+product, are fp16 pairs, whose low part is cut at the step 2^-24 of the smallest numbers,
+so each may be off by 2^-38 of the largest one, which is at most the largest scale times
+the largest weight; times |code| (fp16: |v|) up to 127, while a row of 64 random codes
+holds one above 63, so at most 2 max |v|, over a total of at least the largest weight:
 n 2^-36 max |v|.
 """
 import numpy as np
@@ -55,6 +56,12 @@ class Held:
     def cache(self):
         s = [None if t is None else t.data_ptr() for t in self.scales]
         return rn.Cache.view(self.format, *self.shape[:3], self.codes[0].data_ptr(), self.codes[1].data_ptr(), *s)
+
+    def log_scale(self, b, h, length):
+        """The largest |log2| of a value row's scale."""
+        if self.scales[1] is None or not length:
+            return 0.0
+        return float(torch.log2(self.scales[1][b, h, :length].clamp(min=2.0 ** -100)).abs().max())
 
     def doubles(self, b, h, length):
         out = []
@@ -97,6 +104,8 @@ def check(got, q, prefix, prefix_length, own, lengths=None, counts=None, window=
             if own:
                 parts.append(own.doubles(b, h, lengths[b]))
             k, v = (torch.cat([p[i] for p in parts]) for i in range(2))
+            logs = max(prefix.log_scale(0, h, prefix_length) if prefix_length else 0.0,
+                       own.log_scale(b, h, lengths[b]) if own else 0.0)
             for i in range(counts[b]):
                 end = prefix_length + lengths[b] - counts[b] + i + 1
                 first = max(0, end - window) if window else 0
@@ -110,8 +119,8 @@ def check(got, q, prefix, prefix_length, own, lengths=None, counts=None, window=
                 want = torch.matmul(p, vs)
                 a = scale * torch.matmul(x.abs(), ks.abs().T).amax(-1, keepdim=True)
                 floor = 64 * 2.0 ** -24 * scale * x.abs().amax(-1, keepdim=True) * ks.abs().max()
-                ds = a * (2.0 ** -20 + 134 * 1.5 * 2.0 ** -24) + floor
-                dw = 2.0 ** -22 + 2.0 ** -24 + 2.0 ** -20
+                ds = a * (2.0 ** -20 + 134 * 1.5 * 2.0 ** -24) + floor + 6 * 0.7 * logs * 2.0 ** -24
+                dw = 2.0 ** -22 + 2.0 ** -23 + 2.0 ** -20
                 dn = 2 * (end - first + 64) * 2.0 ** -24
                 bound = torch.matmul(p, vs.abs()) * (2 * ds + dw + dn) + (end - first) * 2.0 ** -36 * vs.abs().max()
                 off = (rows - want).abs()
@@ -168,6 +177,41 @@ def test_drafted_queries(n, t, heads, kv, prefix, capacity, window, format):
 
 
 @pytest.mark.parametrize("format", [I8, F16])
+@pytest.mark.parametrize("window", [0, 1100, 150])
+@pytest.mark.parametrize("n,t,heads,kv", [
+    (1, 1, 2, 2), (1, 3, 4, 4), (5, 1, 4, 2), (1, 12, 2, 2), (20, 1, 2, 2), (2, 10, 2, 2), (1, 30, 1, 1), (40, 1, 2, 2),
+    (4, 12, 3, 3), (2, 30, 2, 2), (70, 1, 4, 4), (6, 12, 2, 2), (4, 33, 2, 2), (9, 1, 64, 1), (130, 1, 16, 8)])
+def test_a_prefix_shared_by_few_and_many_rows(n, t, heads, kv, window, format):
+    """A prefix that is split over blocks, beside own caches: 1 to 576 rows of it a key head,
+    1 to 64 of an own cache."""
+    rng = np.random.default_rng(n + t)
+    prefix, capacity = 1133, 150
+    q, p, o = made(rng, n, t, heads, kv, prefix, capacity, (format, format))
+    lengths = rng.integers(0, capacity + 1, n)
+    lengths[0] = capacity
+    if n > 2:
+        lengths[1], lengths[2] = 0, 1
+    lengths, counts = ints(lengths), ints(rng.integers(0, t + 1, n) if t > 1 and n > 1 else [t] * n)
+    got = attend(q, p, prefix, o, lengths, counts, window)
+    check(got, q, p, prefix, o, lengths, counts, window)
+    assert torch.equal(got, attend(q, p, prefix, o, lengths, counts, window)), "the same call twice"
+
+
+@pytest.mark.parametrize("format", [I8, F16])
+def test_windows_wider_than_everything(format):
+    rng = np.random.default_rng(21)
+    for prefix in (40, 1200):
+        q, p, o = made(rng, 3, 2, 4, 2, prefix, 90, (format, format))
+        lengths = ints([90, 0, 31])
+        want = attend(q, p, prefix, o, lengths)
+        for window in (prefix + 90, 1 << 26, 2 ** 31 - 1):
+            got = attend(q, p, prefix, o, lengths, None, window)
+            check(got, q, p, prefix, o, lengths, None, window)
+            if window > 1 << 26:
+                assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("format", [I8, F16])
 def test_prefix_alone_and_own_alone(format):
     rng = np.random.default_rng(3)
     for n, t, prefix in ((1, 1, 1), (4, 1, 700), (2, 6, 4), (90, 1, 333)):
@@ -198,26 +242,57 @@ def test_queries_of_any_size(size, format):
     check(attend(q, p, 150, o, lengths), q, p, 150, o, lengths)
 
 
-def test_value_scales_of_any_size():
+@pytest.mark.parametrize("prefix", [400, 1400])
+def test_value_scales_of_any_size(prefix):
     """Value rows whose scales differ by many powers of two, growing and falling; zero rows."""
     rng = np.random.default_rng(7)
     for spread in (8.0, 40.0):
         q, _, _ = made(rng, 4, 1, 4, 2, 0, 0, (I8, I8))
-        p, o = Held(I8, 1, 2, 400, rng, spread), Held(I8, 4, 2, 300, rng, spread)
+        p, o = Held(I8, 1, 2, prefix, rng, spread), Held(I8, 4, 2, 300, rng, spread)
         p.scales[1][0, 0] = torch.sort(p.scales[1][0, 0]).values
         p.scales[1][0, 1] = torch.sort(p.scales[1][0, 1], descending=True).values
         o.scales[1][1] = 0.0
         lengths = ints([300, 130, 1, 257])
-        check(attend(q, p, 400, o, lengths), q, p, 400, o, lengths)
+        check(attend(q, p, prefix, o, lengths), q, p, prefix, o, lengths)
+
+
+@pytest.mark.parametrize("prefix", [100, 1400])
+@pytest.mark.parametrize("n,t", [(3, 1), (3, 7), (12, 2)])
+def test_value_scales_that_are_none(n, t, prefix):
+    """Scales below 2^-100 are 0, whatever the codes; negative, infinite ones and NaN make
+    their own rows' outputs NaN and no others, where they are not seen nothing."""
+    rng = np.random.default_rng(22)
+    q, p, o = made(rng, n, t, 4, 2, prefix, 80, (I8, I8))
+    lengths = ints([80] + [50] * (n - 1))
+    p.scales[1][0, 0, 5:70] = 0.0
+    p.scales[1][0, 1, 7] = 2.0 ** -101
+    o.scales[1][0, 0, 3:9] = 2.0 ** -120
+    o.scales[1][1, 1, :] = 0.0
+    got = attend(q, p, prefix, o, lengths)
+    for held in (p, o):
+        held.scales[1][held.scales[1] < 2.0 ** -100] = 0.0
+    assert torch.equal(got, attend(q, p, prefix, o, lengths))
+    check(got, q, p, prefix, o, lengths)
+    for value in (-0.02, float("inf"), -float("inf"), float("nan")):
+        o.scales[1][0, 1, 79] = value   # the last position of sequence 0: its last query's alone
+        o.scales[1][1, 0, 50:] = value  # behind the length
+        p.scales[1][0, 1, prefix] = value
+        bad = attend(q, p, prefix, o, lengths)
+        assert torch.isnan(bad[0, t - 1, 2:]).all()
+        rest = torch.ones((n, t, 4), dtype=torch.bool, device=DEV)
+        rest[0, t - 1, 2:] = False
+        assert torch.equal(bad[rest], got[rest])
 
 
 @pytest.mark.parametrize("format", [I8, F16])
-def test_what_is_not_seen_does_not_matter(format):
+@pytest.mark.parametrize("prefix", [200, 1300])
+@pytest.mark.parametrize("heads", [4, 12, 44])
+def test_what_is_not_seen_does_not_matter(heads, prefix, format):
     """NaN and infinities behind a sequence's length, before a window and in drafted
     positions after a query: the rows that do not see them are as without them, and
     those that do are NaN or infinite."""
     rng = np.random.default_rng(8)
-    n, t, heads, kv, prefix, capacity = 3, 3, 4, 2, 200, 100
+    n, t, kv, capacity = 3, 3, 2, 100
     q, p, o = made(rng, n, t, heads, kv, prefix, capacity, (format, format))
     lengths, counts, window = ints([60, 80, 3]), ints([3, 3, 2]), 90
     clean = attend(q, p, prefix, o, lengths, counts, window)
@@ -242,8 +317,8 @@ def test_what_is_not_seen_does_not_matter(format):
         spoil(oo, 2, 0, 2, value)
         got = attend(q, pp, prefix, oo, lengths, counts, window)
         sees = torch.zeros((n, t, heads), dtype=torch.bool, device=DEV)
-        sees[1, 2, 2:] = True
-        sees[2, 1, :2] = True
+        sees[1, 2, heads // 2:] = True
+        sees[2, 1, :heads // 2] = True
         assert torch.equal(got[~sees], clean[~sees])
         assert (~torch.isfinite(got[sees])).any(-1).all()
 
@@ -267,7 +342,7 @@ def test_values_alone_that_are_not_finite():
 
 def test_bad_numbers_give_nan_in_their_sequence_alone():
     rng = np.random.default_rng(10)
-    for prefix in (0, 50):
+    for prefix in (0, 50, 1000):
         for capacity in (40, 0):
             if not prefix and not capacity:
                 continue
@@ -318,7 +393,8 @@ def test_own_stream_two_graphs_and_changed_lengths():
     other lengths and queries every time, against eager calls."""
     rng = np.random.default_rng(12)
     calls = []
-    for n, t, heads, kv, prefix, capacity in ((6, 1, 8, 8, 300, 90), (3, 4, 12, 4, 70, 200)):
+    for n, t, heads, kv, prefix, capacity in ((6, 1, 8, 8, 300, 90), (3, 4, 12, 4, 70, 200), (6, 1, 8, 8, 2000, 90),
+                                             (5, 4, 12, 4, 1500, 200)):
         q, p, o = made(rng, n, t, heads, kv, prefix, capacity, (I8, I8))
         lengths, out = ints([t] * n), torch.zeros_like(q)
         size = rn.attend_shared_workspace(n, t, heads, p.cache(), prefix, o.cache())

@@ -89,8 +89,9 @@ def test_attend_shared():
     refused(attend(q_stride=255), "q_stride")
     refused(attend(out_stride=252), "q_stride")
     refused(attend(q_stride=258), "q_stride")
-    refused(attend(workspace=None), "workspace")
-    refused(attend(workspace_bytes=64), "workspace")
+    long = cache(sequences=1, capacity=4096)  # (a short prefix needs no workspace)
+    refused(attend(prefix=long, prefix_length=4000, workspace=None), "workspace")
+    refused(attend(prefix=long, prefix_length=4000, workspace_bytes=64), "workspace")
     assert attend(sequences=0, q=None, out=None, workspace=None, workspace_bytes=0) == rn.RN_OK
     assert attend(queries=0, q=None, out=None, workspace=None, workspace_bytes=0) == rn.RN_OK
 
