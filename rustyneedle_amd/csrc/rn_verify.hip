@@ -11,8 +11,9 @@
 // The border of a draw lies between sums of thousands of weights: in 32 bits about one
 // draw in a hundred would depend on the order of additions. The logits are read in 32
 // bits, and exponentials, sums and the comparison are 64-bit, so that the answer is the
-// formula's. A 64-bit exponential is 15 operations here, at the full rate of this
-// chip's vector units, which keeps the pass over the logits bound by memory.
+// formula's. A weight and its sum are 16 instructions, at the full rate of this chip's
+// vector units, which keeps the pass over the logits bound by memory: 285 MB, 64
+// sequences of 8 drafts over 65536, in 59 us (4.8 TB/s, a copy's rate).
 //
 // First every row's maximum and sum by chunks (the only pass over all rows), then the
 // accepted run and the draw: one block a sequence for vocabularies up to 8192, else
@@ -65,11 +66,18 @@ struct Verdict {
     int32_t spare;
 };
 
-// 2^y for -1000 <= y <= 0, relative error below 1.1e-12: y = n + r, |r| <= 1/2, 2^r by
-// its interpolation of degree 8 at the Chebyshev nodes of that interval (exact at 0),
-// n added to the exponent. n comes from the low bits of y + 1.5 2^52.
-__device__ __forceinline__ double exp2_64(double y) {
-    const double t = y + 0x1.8p+52, r = y - (t - 0x1.8p+52);
+// exp((x - peak) / T) with warm = log2(e) / T and least = least_of(warm). What is less
+// than 2^-1000, a masked logit among it, comes out as 2^-1000, which no sum of a row
+// notices (its peak's is 1); a weight counts from kLeast on.
+// 2^y, y = (x - peak) warm, relative error below 1.1e-12: y = n + r, |r| <= 1/2, 2^r by
+// its interpolation of degree 8 at the Chebyshev nodes of that interval (exact at 0);
+// n is the low bits of y + 1.5 2^52. 15 instructions with the sum's (v_ldexp_f64
+// instead of an addition to the exponent, which took five, and y never by itself: 20
+// before that, and the pass over 64 x 17 rows of 65536 63 us, as now 59).
+__device__ __forceinline__ double least_of(double warm) { return -1000.0 / warm; }
+__device__ __forceinline__ double weight(float x, double peak, double warm, double least) {
+    const double d = __builtin_fmax((double)x - peak, least);
+    const double t = __builtin_fma(d, warm, 0x1.8p+52), r = __builtin_fma(d, warm, -(t - 0x1.8p+52));
     double p = 0x1.63d1363a681b4p-20;
     p = __builtin_fma(p, r, 0x1.00dc4a5344ef5p-16);
     p = __builtin_fma(p, r, 0x1.4308ac85a69f8p-13);
@@ -79,21 +87,12 @@ __device__ __forceinline__ double exp2_64(double y) {
     p = __builtin_fma(p, r, 0x1.ebfbdff823cedp-3);
     p = __builtin_fma(p, r, 0x1.62e42fef84cf0p-1);
     p = __builtin_fma(p, r, 1.0);
-    const uint64_t bits = (uint64_t)__double_as_longlong(p);
-    const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)(uint64_t)__double_as_longlong(t) << 20);
-    return __longlong_as_double((long long)(((uint64_t)hi << 32) | (uint32_t)bits));
-}
-
-// exp((x - peak) / T) with warm = log2(e) / T. What is less than 2^-1000, a masked
-// logit among it, comes out as 2^-1000, which no sum of a row notices (its peak's is
-// 1); a weight counts from kLeast on.
-__device__ __forceinline__ double weight(float x, double peak, double warm) {
-    return exp2_64(__builtin_fmax(((double)x - peak) * warm, -1000.0));
+    return __builtin_ldexp(p, (int)(uint32_t)(uint64_t)__double_as_longlong(t));
 }
 constexpr double kLeast = 0x1p-990;  // of one index; 2^24 masked ones sum up to less than kMost
 constexpr double kMost = 0x1p-970;
-__device__ __forceinline__ double likely(float x, double peak, double warm) {
-    const double w = weight(x, peak, warm);
+__device__ __forceinline__ double likely(float x, double peak, double warm, double least) {
+    const double w = weight(x, peak, warm, least);
     return w < kLeast ? 0.0 : w;
 }
 
@@ -182,19 +181,18 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
 #pragma unroll
     for (int e = 0; e < E; ++e) load_logits(row, (chunk * E + e) * kThreads * 4 + t * 4, p.vocab, x[e]);
     float peak = -__builtin_inff();
-    bool bad = false;
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            peak = fmaxf(peak, x[e][c]);
-            bad = bad || !(x[e][c] < __builtin_inff());
+            peak = __builtin_elementwise_maximum(peak, x[e][c]);
         }
     __shared__ float peaks[4];
     __shared__ double sums[4];
     __shared__ uint64_t keys[4];
     __shared__ int bads[4];
     const int wave = t / 64;
+    const bool bad = !(peak < __builtin_inff());  // a NaN wins
     peak = wave_max(peak);
     if (t % 64 == 0) peaks[wave] = peak;
     __syncthreads();
@@ -204,11 +202,11 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
     if (temperature > 0.0f) {
         // a chunk of masked logits has no sum; elsewhere their 2^-1000 do not matter
         if (peak > -__builtin_inff()) {
-            const double warm = kLog2e / (double)temperature;
+            const double warm = kLog2e / (double)temperature, least = least_of(warm);
 #pragma unroll
             for (int e = 0; e < E; ++e)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) sum += weight(x[e][c], (double)peak, warm);
+                for (int c = 0; c < 4; ++c) sum += weight(x[e][c], (double)peak, warm, least);
             sum = wave_sum(sum);
         }
     } else {
@@ -247,7 +245,7 @@ constexpr int kMaxDrafts = 63;  // a lane each, and one for the draw
 // The weights of the draw at four logits, times the sum of the target's row: what is
 // left of p, and p.
 struct Draw {
-    double warm, p_peak, q_peak, ratio;
+    double warm, least, p_peak, q_peak, ratio;
     const float* p_row;
     const float* q_row;  // null: nothing is taken off but `token`
     int token;           // taken off p where there are no draft logits; -1: none
@@ -264,11 +262,11 @@ struct Draw {
     }
     __device__ __forceinline__ void of(int i, const float* x, const float* y, double* rest, double* all) const {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) rest[c] = all[c] = weight(x[c], p_peak, warm);
+        for (int c = 0; c < 4; ++c) rest[c] = all[c] = weight(x[c], p_peak, warm, least);
         if (q_row) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                rest[c] = __builtin_fmax(__builtin_fma(-weight(y[c], q_peak, warm), ratio, all[c]), 0.0);
+                rest[c] = __builtin_fmax(__builtin_fma(-weight(y[c], q_peak, warm, least), ratio, all[c]), 0.0);
         } else if (token >= 0) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -280,6 +278,7 @@ struct Draw {
 __device__ __forceinline__ Draw draw_of(const VerifyParams& p, int b, const Verdict& v, float temperature) {
     Draw d;
     d.warm = kLog2e / (double)temperature;
+    d.least = least_of(d.warm);
     d.p_peak = (double)v.p_peak;
     d.q_peak = (double)v.q_peak;
     d.ratio = v.ratio;
@@ -315,7 +314,7 @@ __device__ __forceinline__ Verdict judge(const VerifyParams& p, int b, float& te
         x = row_of(p, b, lane)[token];
         if (p.draft) y = row_of(p, b, p.drafts + 1 + lane)[token];
     }
-    const double warm = greedy ? 0.0 : kLog2e / (double)temperature;
+    const double warm = greedy ? 1.0 : kLog2e / (double)temperature, least = least_of(warm);
     // ---- every row's total, eight lanes a row
     for (int r = t / 8; r < p.rows; r += THREADS / 8) {
         if (r > p.drafts ? r - p.drafts - 1 >= count : r > count) continue;
@@ -332,10 +331,10 @@ __device__ __forceinline__ Verdict judge(const VerifyParams& p, int b, float& te
                 key = part.key > key ? part.key : key;
                 peak = fmaxf(peak, part.peak);
             } else if (part.peak > peak) {
-                total = total * likely(peak, part.peak, warm) + part.sum;
+                total = total * likely(peak, part.peak, warm, least) + part.sum;
                 peak = part.peak;
             } else if (part.peak > -__builtin_inff()) {
-                total += part.sum * likely(part.peak, peak, warm);
+                total += part.sum * likely(part.peak, peak, warm, least);
             }
         }
         const float most = row8_max(peak);
@@ -347,7 +346,7 @@ __device__ __forceinline__ Verdict judge(const VerifyParams& p, int b, float& te
             key = max_with_dpp_u64<0x4e>(key);
             key = max_with_dpp_u64<0x141>(key);
         } else {
-            total = row8_sum(peak > -__builtin_inff() ? total * likely(peak, most, warm) : 0.0);
+            total = row8_sum(peak > -__builtin_inff() ? total * likely(peak, most, warm, least) : 0.0);
         }
         if (lane % 8 == 0) {
             rows.totals[r] = total;
@@ -376,9 +375,9 @@ __device__ __forceinline__ Verdict judge(const VerifyParams& p, int b, float& te
                     chance = token == rows.firsts[lane] ? 1.0 : 0.0;
                     state = token == rows.firsts[lane] ? 0 : 1;
                 } else {
-                    chance = likely(x, rows.peaks[lane], warm) * rows.inverse[lane];
+                    chance = likely(x, rows.peaks[lane], warm, least) * rows.inverse[lane];
                     double q = 1.0;
-                    if (p.draft) q = likely(y, rows.peaks[dr], warm) * rows.inverse[dr];
+                    if (p.draft) q = likely(y, rows.peaks[dr], warm, least) * rows.inverse[dr];
                     state = (double)u * q < chance ? 0 : 1;
                 }
             }
