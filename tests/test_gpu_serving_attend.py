@@ -176,17 +176,17 @@ def test_drafted_queries(n, t, heads, kv, prefix, capacity, window, format):
     check(got, q, p, prefix, o, lengths, counts, window)
 
 
-@pytest.mark.parametrize("format", [I8, F16])
+@pytest.mark.parametrize("formats", [(I8, I8), (F16, F16), (F16, I8), (I8, F16)])
 @pytest.mark.parametrize("window", [0, 1100, 150])
 @pytest.mark.parametrize("n,t,heads,kv", [
-    (1, 1, 2, 2), (1, 3, 4, 4), (5, 1, 4, 2), (1, 12, 2, 2), (20, 1, 2, 2), (2, 10, 2, 2), (1, 30, 1, 1), (40, 1, 2, 2),
+    (1, 1, 2, 2), (1, 3, 4, 4), (1, 7, 2, 2), (5, 1, 4, 2), (1, 12, 2, 2), (20, 1, 2, 2), (2, 10, 2, 2), (1, 30, 1, 1), (40, 1, 2, 2),
     (4, 12, 3, 3), (2, 30, 2, 2), (70, 1, 4, 4), (6, 12, 2, 2), (4, 33, 2, 2), (9, 1, 64, 1), (130, 1, 16, 8)])
-def test_a_prefix_shared_by_few_and_many_rows(n, t, heads, kv, window, format):
+def test_a_prefix_shared_by_few_and_many_rows(n, t, heads, kv, window, formats):
     """A prefix that is split over blocks, beside own caches: 1 to 576 rows of it a key head,
     1 to 64 of an own cache."""
     rng = np.random.default_rng(n + t)
     prefix, capacity = 1133, 150
-    q, p, o = made(rng, n, t, heads, kv, prefix, capacity, (format, format))
+    q, p, o = made(rng, n, t, heads, kv, prefix, capacity, formats)
     lengths = rng.integers(0, capacity + 1, n)
     lengths[0] = capacity
     if n > 2:
@@ -219,6 +219,29 @@ def test_prefix_alone_and_own_alone(format):
         check(attend(q, p, prefix, None), q, p, prefix, None)
     q, _, o = made(rng, 5, 2, 4, 2, 0, 77, (format, format))
     check(attend(q, None, 0, o), q, None, 0, o)  # every sequence full
+
+
+def test_nothing_to_see_gives_zeros():
+    """An empty prefix without own caches, and own caches of no rows."""
+    rng = np.random.default_rng(23)
+    q, p, o = made(rng, 3, 2, 4, 2, 20, 30, (I8, I8))
+    assert (attend(q, p, 0, None) == 0).all()
+    assert (attend(q, None, 0, o, ints([0, 0, 0])) == 0).all()
+    assert (attend(q, p, 0, o, ints([0, 0, 0])) == 0).all()
+    got = attend(q, p, 1, o, ints([0, 0, 0]))  # the first query stands before the first position
+    assert (got[:, 0] == 0).all()
+    check(got, q, p, 1, o, ints([0, 0, 0]))
+
+
+@pytest.mark.parametrize("format", [I8, F16])
+@pytest.mark.parametrize("prefix", [0, 100, 1500])
+def test_a_prompt_in_one_call(prefix, format):
+    """Hundreds of queries a sequence, each seeing up to its own position."""
+    rng = np.random.default_rng(24)
+    q, p, o = made(rng, 2, 333, 4, 2, prefix, 400, (format, format))
+    lengths, counts = ints([400, 200]), ints([333, 200])
+    got = attend(q, p, prefix, o, lengths, counts)
+    check(got, q, p, prefix, o, lengths, counts)
 
 
 @pytest.mark.parametrize("format", [I8, F16])
