@@ -216,7 +216,7 @@ struct Share {
     const float *key_scales, *value_scales;
 };
 
-template <bool I8, int TILE>
+template <bool I8, class Of>
 __device__ __forceinline__ Share share_of(const SharedParams& p, bool prefix, bool all, int sequence, int head, int tile,
                                           int split, int splits, int slot) {
     const CacheDev& cache = prefix ? p.prefix : p.own;
@@ -231,13 +231,19 @@ __device__ __forceinline__ Share share_of(const SharedParams& p, bool prefix, bo
         s.first = p.prefix_first;
         s.last = p.prefix_length;
     } else {
+        // from the first position that the tile's first query sees to its last one's own
         const Sequence q = sequence_of(p, sequence);
-        const int seen = p.prefix_length + q.length - q.count + 1 - p.window;  // the first query's first position
-        s.last = uniform(prefix ? p.prefix_length : q.length);
-        s.first = uniform(p.window > 0 ? max(min(seen - s.origin, s.last), 0) : 0);
+        int t0 = 0, t1 = q.count;
+        if (p.own_tiles > 1) {
+            t0 = quotient(tile * Of::kRows, p.group);
+            t1 = min(t1, quotient(tile * Of::kRows + Of::kRows - 1, p.group) + 1);
+        }
+        const int before = p.prefix_length + q.length - q.count - s.origin;
+        s.last = uniform(t1 > t0 ? max(min(before + t1, prefix ? p.prefix_length : q.length), 0) : 0);
+        s.first = uniform(p.window > 0 ? max(min(before + t0 + 1 - p.window, s.last), 0) : 0);
     }
     // (at most 2^19 tiles times 4096 shares)
-    const uint32_t tiles = (uint32_t)(s.last - s.first + TILE - 1) / TILE;
+    const uint32_t tiles = (uint32_t)(s.last - s.first + Of::kKeys - 1) / Of::kKeys;
     s.t0 = uniform((int)(tiles * (uint32_t)split / (uint32_t)splits));
     s.t1 = uniform((int)(tiles * (uint32_t)(split + 1) / (uint32_t)splits));
     const int64_t base = (prefix ? 0 : (int64_t)sequence * cache.sequence_rows) + (int64_t)head * cache.head_rows;
@@ -248,9 +254,9 @@ __device__ __forceinline__ Share share_of(const SharedParams& p, bool prefix, bo
     return s;
 }
 
-template <bool I8, int TILE>
+template <bool I8, class Of>
 __device__ __forceinline__ Share own_share(const SharedParams& p, int sequence, int head, int tile, int split) {
-    return share_of<I8, TILE>(p, false, false, sequence, head, tile, split, p.own_splits, p.prefix_splits + split);
+    return share_of<I8, Of>(p, false, false, sequence, head, tile, split, p.own_splits, p.prefix_splits + split);
 }
 
 // Row number r of the block's rows: where its query lies (null: there is none). What
@@ -744,7 +750,7 @@ struct Job {
         for (int d = 0; d < kWide; ++d) acc[d] = vacc{};
         pass(f);
         if constexpr (BOTH) {
-            st.share = own_share<I8, kKeys>(p, st.share.sequence, st.share.head, st.share.tile, 0);
+            st.share = own_share<I8, Job>(p, st.share.sequence, st.share.head, st.share.tile, 0);
             if (st.share.t0 < st.share.t1) st.fetch(0, f);
             own_limits(p, row);
             st.sync();
@@ -1043,7 +1049,7 @@ struct FewJob {
         for (int d = 0; d < 4; ++d) acc[d] = v4f{0, 0, 0, 0};
         pass(f);
         if constexpr (BOTH) {
-            share = own_share<I8, kKeys>(p, share.sequence, share.head, share.tile, 0);
+            share = own_share<I8, FewJob>(p, share.sequence, share.head, share.tile, 0);
             if (share.t0 + wave < share.t1) fetch(share.t0 + wave, f);
             own_limits(p, row);
             pass(f);
@@ -1107,12 +1113,12 @@ __global__ __launch_bounds__(256, (blocks_a_cu<I8, QP, WP, QO>())) void shared_a
     if (prefix) {
         const int share = uniform(quotient(rest, p.prefix_tiles)), tile = rest - share * p.prefix_tiles;
         const int head = uniform(quotient(share, p.prefix_splits)), split = share - head * p.prefix_splits;
-        Prefix(p, share_of<I8, Prefix::kKeys>(p, true, true, 0, head, tile, split, p.prefix_splits, split), lds).template run<false>();
+        Prefix(p, share_of<I8, Prefix>(p, true, true, 0, head, tile, split, p.prefix_splits, split), lds).template run<false>();
     } else {
         const int share = uniform(quotient(rest, p.own_tiles)), tile = rest - share * p.own_tiles;
         const int pair = uniform(quotient(share, p.own_splits)), split = share - pair * p.own_splits;
         const int sequence = uniform(quotient(pair, p.kv_heads)), head = pair - sequence * p.kv_heads;
-        Own(p, own_share<I8, Own::kKeys>(p, sequence, head, tile, split), lds).template run<false>();
+        Own(p, own_share<I8, Own>(p, sequence, head, tile, split), lds).template run<false>();
         if (!p.parts) refuse(p, sequence);
     }
 }
@@ -1125,7 +1131,7 @@ __global__ __launch_bounds__(256, (blocks_a_cu<I8, Q, 1, Q>())) void alone_atten
     __shared__ __attribute__((aligned(16))) char lds[Rows::kLds];
     const int pair = uniform(quotient(blockIdx.x, p.own_tiles)), tile = blockIdx.x - pair * p.own_tiles;
     const int sequence = uniform(quotient(pair, p.kv_heads)), head = pair - sequence * p.kv_heads;
-    Rows(p, share_of<I8, Rows::kKeys>(p, true, false, sequence, head, tile, 0, 1, 0), lds).template run<true>();
+    Rows(p, share_of<I8, Rows>(p, true, false, sequence, head, tile, 0, 1, 0), lds).template run<true>();
     refuse(p, sequence);
 }
 
