@@ -13,7 +13,7 @@
 // bits, and exponentials, sums and the comparison are 64-bit, so that the answer is the
 // formula's. A weight and its sum are 16 instructions, at the full rate of this chip's
 // vector units, which keeps the pass over the logits bound by memory: 285 MB, 64
-// sequences of 8 drafts over 65536, in 59 us (4.8 TB/s, a copy's rate).
+// sequences of 8 drafts over 65536, in 55 us (5.2 TB/s; a copy reaches 4.9).
 //
 // First every row's maximum and sum by chunks (the only pass over all rows), then the
 // accepted run and the draw: one block a sequence for vocabularies up to 8192, else
@@ -39,10 +39,10 @@ struct VerifyParams {
     int32_t* emitted;       // [sequences][drafts + 1]
     float* probabilities;
     int32_t* error;
-    struct RowPart* parts;   // [sequences][rows a sequence][chunks]
+    struct RowPart* parts;   // [sequences][rows a sequence][row_parts]
     double2* sums;           // [sequences][chunks]: of the drawn row's rest, and of p
     struct Verdict* verdicts;  // [sequences]
-    int sequences, drafts, vocab, rows, chunks, span;
+    int sequences, drafts, vocab, rows, row_parts, chunks, span;
 };
 
 // One chunk of one row: the sum of exp((x - peak) / T), the peak; at temperature 0 the
@@ -66,15 +66,17 @@ struct Verdict {
     int32_t spare;
 };
 
-// exp((x - peak) / T) with warm = log2(e) / T and least = least_of(warm). What is less
+constexpr double kLog2e = 1.4426950408889634;
+
+// exp((x - peak) / T) with warm = log2(e) / T and least = least_of(temperature). What is less
 // than 2^-1000, a masked logit among it, comes out as 2^-1000, which no sum of a row
 // notices (its peak's is 1); a weight counts from kLeast on.
 // 2^y, y = (x - peak) warm, relative error below 1.1e-12: y = n + r, |r| <= 1/2, 2^r by
 // its interpolation of degree 8 at the Chebyshev nodes of that interval (exact at 0);
 // n is the low bits of y + 1.5 2^52. 15 instructions with the sum's (v_ldexp_f64
 // instead of an addition to the exponent, which took five, and y never by itself: 20
-// before that, and the pass over 64 x 17 rows of 65536 63 us, as now 59).
-__device__ __forceinline__ double least_of(double warm) { return -1000.0 / warm; }
+// before that, and the pass over 64 x 17 rows of 65536 63 us, 59 then).
+__device__ __forceinline__ double least_of(float temperature) { return -1000.0 / kLog2e * (double)temperature; }
 __device__ __forceinline__ double weight(float x, double peak, double warm, double least) {
     const double d = __builtin_fmax((double)x - peak, least);
     const double t = __builtin_fma(d, warm, 0x1.8p+52), r = __builtin_fma(d, warm, -(t - 0x1.8p+52));
@@ -141,8 +143,6 @@ __device__ __forceinline__ double wave_scan(double v) {
     return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
 }
 
-constexpr double kLog2e = 1.4426950408889634;
-
 // Four consecutive logits of a row at i (-infinity past its end); rows need no more
 // than the alignment of a float.
 __device__ __forceinline__ void load_logits(const float* row, int i, int vocab, float* x) {
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
     if (temperature > 0.0f) {
         // a chunk of masked logits has no sum; elsewhere their 2^-1000 do not matter
         if (peak > -__builtin_inff()) {
-            const double warm = kLog2e / (double)temperature, least = least_of(warm);
+            const double warm = kLog2e / (double)temperature, least = least_of(temperature);
 #pragma unroll
             for (int e = 0; e < E; ++e)
 #pragma unroll
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
         }
         out.peak = peak;
         out.bad = bads[0] | bads[1] | bads[2] | bads[3];
-        p.parts[((int64_t)b * p.rows + r) * p.chunks + chunk] = out;
+        p.parts[((int64_t)b * p.rows + r) * p.row_parts + chunk] = out;
     }
 }
 
@@ -278,7 +278,7 @@ struct Draw {
 __device__ __forceinline__ Draw draw_of(const VerifyParams& p, int b, const Verdict& v, float temperature) {
     Draw d;
     d.warm = kLog2e / (double)temperature;
-    d.least = least_of(d.warm);
+    d.least = least_of(temperature);
     d.p_peak = (double)v.p_peak;
     d.q_peak = (double)v.q_peak;
     d.ratio = v.ratio;
@@ -314,17 +314,17 @@ __device__ __forceinline__ Verdict judge(const VerifyParams& p, int b, float& te
         x = row_of(p, b, lane)[token];
         if (p.draft) y = row_of(p, b, p.drafts + 1 + lane)[token];
     }
-    const double warm = greedy ? 1.0 : kLog2e / (double)temperature, least = least_of(warm);
+    const double warm = greedy ? 1.0 : kLog2e / (double)temperature, least = least_of(temperature);
     // ---- every row's total, eight lanes a row
     for (int r = t / 8; r < p.rows; r += THREADS / 8) {
         if (r > p.drafts ? r - p.drafts - 1 >= count : r > count) continue;
-        const RowPart* parts = p.parts + ((int64_t)b * p.rows + r) * p.chunks;
+        const RowPart* parts = p.parts + ((int64_t)b * p.rows + r) * p.row_parts;
         float peak = -__builtin_inff();
         double total = 0.0;
         int bad = 0;
         uint64_t key = 0;
 #pragma unroll 2
-        for (int c = lane % 8; c < p.chunks; c += 8) {
+        for (int c = lane % 8; c < p.row_parts; c += 8) {
             const RowPart part = parts[c];
             bad |= part.bad;
             if (greedy) {
@@ -605,17 +605,21 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(const VerifyParams
 }
 
 struct VerifyPlan {
-    int rows = 0, each = 1, chunks = 0;  // each: 4-logit loads a thread
+    int rows = 0, each = 1, row_parts = 0, chunks = 0;  // each: 4-logit loads a thread of the pass over all rows
     size_t sums_at = 0, verdicts_at = 0, bytes = 0;
 };
 
 VerifyPlan verify_plan(int sequences, int drafts, int vocab) {
     VerifyPlan n;
     n.rows = 2 * drafts + 1;
-    // 16 logits a thread where that still gives the chip four blocks a CU, else 4
-    n.each = (int64_t)sequences * n.rows * ((vocab + 4095) / 4096) >= 1024 ? 4 : 1;
-    n.chunks = (vocab + 1024 * n.each - 1) / (1024 * n.each);
-    n.sums_at = aligned_bytes((size_t)sequences * n.rows * n.chunks * sizeof(RowPart));
+    // 32 logits a thread where that still gives the chip four blocks a CU, else 16, else 4:
+    // a thread's joins and its 64-bit quotient are about 110 instructions (64 x 17 rows of
+    // 65536: 55 us with 32, 59 with 16; 64 x 9 of 8192, too few for 32: 7.3 with 16)
+    const int64_t all = (int64_t)sequences * n.rows;
+    n.each = all * ((vocab + 8191) / 8192) >= 1024 ? 8 : all * ((vocab + 4095) / 4096) >= 1024 ? 4 : 1;
+    n.row_parts = (vocab + 1024 * n.each - 1) / (1024 * n.each);
+    n.chunks = n.each > 1 ? (vocab + 4095) / 4096 : n.row_parts;
+    n.sums_at = aligned_bytes((size_t)sequences * n.rows * n.row_parts * sizeof(RowPart));
     n.verdicts_at = n.sums_at + aligned_bytes((size_t)sequences * n.chunks * sizeof(double2));
     n.bytes = n.verdicts_at + aligned_bytes((size_t)sequences * sizeof(Verdict));
     return n;
@@ -687,16 +691,20 @@ int rn_verify_drafts(int sequences, int drafts, int vocab, const float* target, 
     p.drafts = drafts;
     p.vocab = vocab;
     p.rows = draft ? n.rows : drafts + 1;
+    p.row_parts = n.row_parts;
     p.chunks = n.chunks;
     // as many chunks a block as leave a block a CU: each block judges the run again
     const int64_t span = (int64_t)sequences * n.chunks / 256;
     p.span = span < 1 ? 1 : span > kSpan ? kSpan : (int)span;
     hipStream_t s = (hipStream_t)stream;
-    const dim3 rows(n.chunks, p.rows, sequences), run((n.chunks + p.span - 1) / p.span, sequences), draw(sequences), block(kThreads);
-    rn_launch(n.each == 4 ? verify_rows_kernel<4> : verify_rows_kernel<1>, rows, block, 0, s, p);
+    const dim3 rows(n.row_parts, p.rows, sequences), run((n.chunks + p.span - 1) / p.span, sequences), draw(sequences), block(kThreads);
+    rn_launch(n.each == 8   ? verify_rows_kernel<8>
+              : n.each == 4 ? verify_rows_kernel<4>
+                            : verify_rows_kernel<1>,
+              rows, block, 0, s, p);
     if (vocab <= kWide * 8) {
         rn_launch(vocab <= kWide * 4 ? verify_finish_kernel<1> : verify_finish_kernel<2>, draw, dim3(kWide), 0, s, p);
-    } else if (n.each == 4) {
+    } else if (n.each > 1) {
         rn_launch(verify_run_kernel<4 * kThreads>, run, dim3(4 * kThreads), 0, s, p);
         rn_launch(verify_draw_kernel<4 * kThreads>, draw, dim3(4 * kThreads), 0, s, p);
     } else {
