@@ -23,11 +23,13 @@
 // where a single one is off by 2e-4. A value row's scale enters the weight's exponent.
 //
 // What bounds it (MI355X, traced): 256 8-bit rows over a prefix of 32768 positions on 8
-// heads, 256 own caches of up to 1024: 75 us and 5 for the join, where own caches alone
-// take 34 us (4.5 TB/s of 4.9) and the prefix 61 (69 GFLOP as fp16 pairs, 32x32x16
-// matrix instructions 45% of the time, the rest exponentials and the splitting of
-// weights, which a matrix instruction leaves 9 cycles of its 34 to no other vector
-// instruction); fp16 own caches of 550 keys: 51 us, 5.6 TB/s.
+// heads and 256 own caches of 550 keys: 75 us and 5 for the join, where own caches alone
+// take 34 us (4.5 TB/s of 4.9) and the prefix 61 (34 GFLOP as fp16 pairs). The vector
+// units issue 54% of that time and the matrix units are busy 23%, and the two overlap
+// only in part: a round of 32 keys and 32 rows a wave is 16 matrix instructions and about
+// 165 others (scales 48, exponentials 32, sums 16, weights as two fp16 numbers 32, the
+// maximum, the next tile), 0.8 us a SIMD with two waves and 0.9 with one. fp16 own
+// caches of 550 keys: 51 us, 5.6 TB/s.
 #include "rn_device.hpp"
 #include "rn_serving.hpp"
 
