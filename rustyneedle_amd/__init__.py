@@ -699,6 +699,9 @@ def attend_heads(q: np.ndarray, K: np.ndarray, V: np.ndarray, lengths: np.ndarra
 
 
 # ---- serving over caller-held caches ---------------------------------------------------
+# Addresses are device memory of any owner: DeviceBuffer, a torch tensor's data_ptr(). A
+# process that uses torch imports it before this package: torch brings a HIP runtime of
+# its own, which the library then shares; the other way round it finds no device.
 
 class Cache:
     """A key/value cache in device memory (rn_cache): 8-bit codes with a scale a row

@@ -3,6 +3,13 @@ import sys
 
 import pytest
 
+# torch brings a HIP runtime of its own; loaded first, the library shares it, while a
+# second one in a process finds no device
+try:
+    import torch  # noqa: F401
+except ImportError:
+    pass
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
