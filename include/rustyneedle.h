@@ -447,13 +447,14 @@ int rn_cache_read(const rn_cache* cache, const rn_cache_rows* rows, int tokens, 
  * scale times q . k, out = sum softmax(score) v; a query that sees nothing gives
  * zeros. Rows past counts[b] stay as they are. Positions a query does not see never
  * reach it, whatever they hold; a NaN or infinity that it sees makes its output so.
- * scale must be positive and finite. Value rows' scales are positive, as rn_cache_write
+ * scale must be positive and below 2.3e38. Value rows' scales are positive, as rn_cache_write
  * leaves them: below 2^-100 they count as 0, negative and infinite ones and NaN make the
  * output of the queries that see them NaN, and those a query sees should lie within
  * 2^116 of one another (zeros aside: below 2^16), or small weights are lost.
  * Products and sums are f32 (queries and weights enter the matrix instructions as
- * pairs of fp16 numbers, 22 bits; relative error about 1e-6); the result depends on
- * the shapes, lengths, counts and window only and repeats bit for bit.
+ * pairs of fp16 numbers, 22 bits; relative error about 1e-6). A row's result depends on
+ * its own query, what it sees, the shapes, lengths, counts and window only, whatever the
+ * other rows hold, and repeats bit for bit.
  * A sequence with lengths[b] outside 0..capacity or counts[b] outside 0..queries gets
  * NaN in all its rows. workspace: workspace_bytes of device memory aligned to 256
  * bytes, at least what rn_attend_shared_workspace says for the same arguments (0 where

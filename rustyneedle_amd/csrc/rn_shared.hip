@@ -651,7 +651,8 @@ struct Job {
         if (__any(m > row.mr + kSlack)) {
             float y = max_of(m, lane_xor<32>(m));
             if constexpr (kParts == 4) y = max_of(y, lane_xor<16>(y));
-            y = max_of(y, row.mr);
+            // (a column by its own scores alone: the others of the tile do not matter to it)
+            y = y > row.mr + kSlack ? y : row.mr;
             const float alpha = exp2_of(row.mr - y);
             row.l = scaled_sum(row.l, row.mr - y);
 #pragma unroll
@@ -961,7 +962,8 @@ struct FewJob {
         if (__any(m > row.mr + kSlack)) {
             float y = max_of(m, lane_xor<16>(m));
             y = max_of(y, lane_xor<32>(y));
-            y = max_of(y, row.mr);
+            // (a column by its own scores alone: the others of the tile do not matter to it)
+            y = y > row.mr + kSlack ? y : row.mr;
             const float alpha = exp2_of(row.mr - y);
             row.l = scaled_sum(row.l, row.mr - y);
 #pragma unroll
@@ -1364,7 +1366,8 @@ int rn_attend_shared(const float* q, int64_t q_stride, float* out, int64_t out_s
     int kv_heads, capacity;
     SV_CHECK(check_shape(sequences, queries, heads, prefix, prefix_length, own, kv_heads, capacity));
     SV_REQUIRE(own || !lengths, "lengths without an own cache");
-    SV_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive and finite");
+    const float scale2 = scale * 1.44269504088896340736f;
+    SV_REQUIRE(scale > 0.0f && scale2 < INFINITY, "scale must be positive and below 2.3e38");
     SV_REQUIRE(window >= 0, "window must not be negative (got %d)", window);
     if (window > (1 << 26)) window = 0;  // wider than any sequence
     if (sequences == 0 || queries == 0) return RN_OK;
@@ -1412,7 +1415,7 @@ int rn_attend_shared(const float* q, int64_t q_stride, float* out, int64_t out_s
     p.prefix_splits = n.prefix_splits;
     p.own_tiles = n.own_tiles;
     p.own_splits = n.own_splits;
-    p.scale2 = scale * 1.44269504088896340736f;
+    p.scale2 = scale2;
     const int64_t shared = (int64_t)kv_heads * n.prefix_tiles * n.prefix_splits;
     const int64_t single = (int64_t)sequences * kv_heads * n.own_tiles * n.own_splits;
     hipStream_t s = (hipStream_t)stream;

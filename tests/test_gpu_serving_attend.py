@@ -253,7 +253,7 @@ def test_long_prefix_and_a_long_own_cache(format):
 
 
 @pytest.mark.parametrize("format", [I8, F16])
-@pytest.mark.parametrize("size", [1e-30, 1e-4, 30.0, 3000.0])
+@pytest.mark.parametrize("size", [1e-42, 1e-30, 1e-4, 30.0, 3000.0])
 def test_queries_of_any_size(size, format):
     """Tiny ones weigh all positions alike, huge ones pick one; a row of zeros among them."""
     rng = np.random.default_rng(6)
@@ -263,6 +263,50 @@ def test_queries_of_any_size(size, format):
     q[3, 0, 1, 5] = size * 1000
     lengths = ints([90, 3, 50, 64, 65, 0])
     check(attend(q, p, 150, o, lengths), q, p, 150, o, lengths)
+
+
+@pytest.mark.parametrize("format", [I8, F16])
+@pytest.mark.parametrize("prefix", [100, 1400])
+@pytest.mark.parametrize("n,t,heads", [(3, 1, 4), (20, 1, 12), (6, 3, 4)])
+def test_a_query_that_is_not_finite_stays_alone(n, t, heads, prefix, format):
+    rng = np.random.default_rng(25)
+    q, p, o = made(rng, n, t, heads, 2, prefix, 60, (format, format))
+    lengths = ints([60] * n)
+    clean = attend(q, p, prefix, o, lengths)
+    for value in (float("nan"), float("inf")):
+        bad = q.clone()
+        bad[1, 0, 1, 7] = value
+        got = attend(bad, p, prefix, o, lengths)
+        assert torch.isnan(got[1, 0, 1]).all()
+        rest = torch.ones((n, t, heads), dtype=torch.bool, device=DEV)
+        rest[1, 0, 1] = False
+        assert torch.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize("format", [I8, F16])
+def test_offsets_past_32_bits(format):
+    """Sequences that lie more than 2^32 bytes apart."""
+    rng = np.random.default_rng(26)
+    apart, n, kv, capacity = (1 << 26) + 3, 2, 2, 50
+    q, p, o = made(rng, n, 1, 4, kv, 70, capacity, (format, format))
+    rows = apart + kv * capacity
+    codes = [torch.empty((rows, 64), dtype=o.codes[0].dtype, device=DEV) for _ in range(2)]
+    scales = [None if x is None else torch.empty((rows,), device=DEV) for x in o.scales]
+    for b in range(n):
+        here = slice(b * apart, b * apart + kv * capacity)
+        for i in range(2):
+            codes[i][here] = o.codes[i][b].reshape(-1, 64)
+            if scales[i] is not None:
+                scales[i][here] = o.scales[i][b].reshape(-1)
+    view = rn.Cache.view(format, n, kv, capacity, codes[0].data_ptr(), codes[1].data_ptr(),
+                         *[None if x is None else x.data_ptr() for x in scales], apart, capacity)
+    lengths = ints([50, 31])
+    want = [attend(q, a, 70 if a else 0, o, lengths) for a in (p, None)]
+    o.cache = lambda: view
+    for a, w in zip((p, None), want):
+        got = attend(q, a, 70 if a else 0, o, lengths)
+        check(got, q, a, 70 if a else 0, o, lengths)
+        assert torch.equal(got, w)
 
 
 @pytest.mark.parametrize("prefix", [400, 1400])

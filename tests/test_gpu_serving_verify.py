@@ -186,6 +186,40 @@ def test_logits_of_any_size(size):
     check((target * size).astype(np.float32), (draft * size).astype(np.float32), tokens, None, temperatures, uniforms)
 
 
+@pytest.mark.parametrize("n,vocab", [(3, 50), (40, 3000), (20, 20000)])
+def test_masks_of_the_lowest_number(n, vocab):
+    """Tokens masked with the lowest float: nothing where others are left, alike where all are."""
+    target, draft, tokens, temperatures, uniforms, rng = made(n, 3, vocab, 31)
+    lowest = np.finfo(np.float32).min
+    out = rng.random(target.shape) < 0.7
+    out[..., vocab // 3] = False
+    target[out] = lowest
+    target[1] = lowest
+    draft[2] = lowest
+    check(target, draft, tokens, None, temperatures, uniforms)
+    check(target, None, tokens, None, temperatures, uniforms)
+
+
+def test_rows_past_32_bits():
+    """Rows of logits that lie more than 2^32 bytes apart."""
+    vocab, apart = 300, (1 << 30) + 1
+    target, draft, tokens, temperatures, uniforms, _ = made(1, 1, vocab, 33)
+    wide = torch.empty((apart + vocab,), device=DEV)
+    for i in range(2):
+        wide[i * apart:i * apart + vocab] = device(target[0, i])
+    q, tok, temp, uni = device(draft), device(tokens), device(temperatures), device(uniforms)
+    accepted = torch.full((1,), -7, dtype=torch.int32, device=DEV)
+    emitted = torch.full((1, 2), -7, dtype=torch.int32, device=DEV)
+    size = rn.verify_drafts_workspace(1, 1, vocab)
+    work = torch.zeros((size,), dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    rn.verify_drafts(1, 1, vocab, wide.data_ptr(), q.data_ptr(), tok.data_ptr(), None, temp.data_ptr(), uni.data_ptr(),
+                     accepted.data_ptr(), emitted.data_ptr(), None, work.data_ptr(), size, apart)
+    torch.cuda.synchronize()
+    a, e, _ = rule(target[0], draft[0], tokens[0], 1, float(temperatures[0]), uniforms[0], vocab)
+    assert accepted.item() == a and emitted[0, :a + 1].tolist() == e
+
+
 def test_what_cannot_be_judged_ends_the_run():
     n, d, vocab = 12, 3, 500
     target, draft, tokens, temperatures, uniforms, _ = made(n, d, vocab, 12)

@@ -81,7 +81,7 @@ def test_attend_shared():
     refused(attend(own=cache(kv_heads=4)), "differ")
     refused(attend(queries=65536), "2^20")
     refused(attend(queries=65535, sequences=2, heads=64, q_stride=4096, out_stride=4096), "2^20")
-    for scale in (0.0, -1.0, float("inf"), float("nan")):
+    for scale in (0.0, -1.0, 3e38, float("inf"), float("nan")):
         refused(attend(scale=scale), "scale")
     refused(attend(window=-1), "window")
     refused(attend(q=None), "null")
