@@ -24,7 +24,7 @@
 //
 // What bounds it (MI355X, traced): 256 8-bit rows over a prefix of 32768 positions on 8
 // heads and 256 own caches of 550 keys: 75 us and 5 for the join, where own caches alone
-// take 34 us (4.5 TB/s of 4.9) and the prefix 61 (34 GFLOP as fp16 pairs). The vector
+// take 33 us (4.6 TB/s of 4.9) and the prefix 61 (34 GFLOP as fp16 pairs). The vector
 // units issue 54% of that time and the matrix units are busy 23%, and the two overlap
 // only in part: a round of 32 keys and 32 rows a wave is 16 matrix instructions and about
 // 165 others (scales 48, exponentials 32, sums 16, weights as two fp16 numbers 32, the
@@ -806,7 +806,7 @@ template <bool I8>
 struct FewJob {
     static constexpr int kTiles = I8 ? 4 : 2, kKeys = 16 * kTiles, kRows = 16 / kTiles, kKeyLoads = 4, kValueLoads = 4;
     static constexpr int kValueBytes = kKeys * (I8 ? 64 : 128);
-    static constexpr int kJoinBytes = 4 * 16 * (kCacheWidth * 4 + 16);
+    static constexpr int kJoinBytes = 4 * kRows * (kCacheWidth * 4 + 16);
     static constexpr int kLds = 4 * kValueBytes > kJoinBytes ? 4 * kValueBytes : kJoinBytes;
 
     const SharedParams& p;
@@ -1059,14 +1059,43 @@ struct FewJob {
             pass(f);
         }
         close_row(row);
+        join_tiles();
         __syncthreads();
         float* sums = reinterpret_cast<float*>(lds);
-        float4* heads = reinterpret_cast<float4*>(lds + 4 * 16 * kCacheWidth * 4);
-        put_column(sums, heads, wave * 16 + col, quad, acc, row);
+        float4* heads = reinterpret_cast<float4*>(lds + 4 * kRows * kCacheWidth * 4);
+        if (kt == 0) put_column(sums, heads, wave * kRows + col / kTiles, quad, acc, row);
         __syncthreads();
         // sixteen threads a row, each of four waves' columns of it
         if (threadIdx.x < kRows * 16)
-            join_columns<4, 16, kTiles>(p, sums, heads, (int)threadIdx.x / 16 * kTiles, threadIdx.x % 16, share.slot);
+            join_columns<4, kRows, 1>(p, sums, heads, (int)threadIdx.x / 16, threadIdx.x % 16, share.slot);
+    }
+
+    template <int CTRL>
+    __device__ __forceinline__ static float neighbour(float v) {
+        return __int_as_float(dpp_move<CTRL>(__float_as_int(v)));
+    }
+    // Joins a row's columns, neighbours among the lanes, in all of them. (Left to the one
+    // wave that joins the four, sixteen columns a row took it 2.5 us: 16 sequences over
+    // 600 positions 11.6 us against 10.5.)
+    __device__ __forceinline__ void join_tiles() {
+        float m = row.l != 0.0f ? row.mr : -__builtin_inff();
+        m = max_of(m, neighbour<0xb1>(m));
+        if constexpr (kTiles == 4) m = max_of(m, neighbour<0x4e>(m));
+        const float a = exp2_of(row.mr - m);
+        const bool some = row.l != 0.0f;
+        row.l = some ? scaled_sum(row.l, row.mr - m) : 0.0f;
+        row.l += neighbour<0xb1>(row.l);
+        if constexpr (kTiles == 4) row.l += neighbour<0x4e>(row.l);
+        row.mr = m;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v = some ? acc[d][j] * a : 0.0f;
+                v += neighbour<0xb1>(v);
+                if constexpr (kTiles == 4) v += neighbour<0x4e>(v);
+                acc[d][j] = v;
+            }
     }
 };
 
@@ -1223,9 +1252,9 @@ Plan plan_of(int sequences, int queries, int heads, const rn_cache* prefix, int 
     const int shared_rows = sequences * queries * group, own_rows = queries * group;
     // A short prefix and few blocks: each reads the prefix for itself, which saves the
     // second launch and the shares (8-bit, 140 keys of their own, alone against shared:
-    // 16 sequences of 3 rows on 4 heads, prefix 256: 8.7 us against 13.1, 600: 10.9
-    // against 13.4, 1500: 14.6 against 13.4; 64 sequences on 8 heads, 600: 14.6 against
-    // 14.0; 256 sequences, 2048 blocks, 256: 26.6 against 23.1).
+    // 16 sequences of 3 rows on 4 heads, prefix 256: 7.9 us against 13.0, 600: 10.6
+    // against 13.4, 1500: 14.5 against 13.5; 64 sequences on 8 heads, 600: 13.5 against
+    // 14.3, 1000: 15.5 against 14.1; 256 sequences, 2048 blocks, 256: 25.1 against 22.5).
     if (prefix_length > 0 && (!own || own->format == prefix->format)) {
         const int few = few_rows(prefix), rows = own_rows <= few ? few : own_rows <= 16 ? 16 : 32;
         const int64_t blocks = (int64_t)sequences * kv_heads * ((own_rows + rows - 1) / rows);
